@@ -10,7 +10,9 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libiggt_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast",
-         "-Wno-unused-result", "-DNDEBUG"]
+         "-Wno-unused-result", "-DNDEBUG",
+         # no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # extra flags of single translation units (measured choices, each explained in the file it applies to)
 PER_FILE_FLAGS = {"attention_v3_est.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]}
 
