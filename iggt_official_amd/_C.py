@@ -14,7 +14,7 @@ _LIB_PATH = os.environ.get("IGGT_HIP_LIB") or os.path.join(os.path.dirname(os.pa
                                                            "libiggt_hip.so")
 _lib = None
 
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 _c_void_p, _c_int, _c_long, _c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 
@@ -131,10 +131,25 @@ _SIGNATURES = {
     "iggt_hdbscan_labels_from_mst": [_c_void_p, _c_void_p, _c_void_p, _c_long, _c_int, ctypes.c_double, _c_int, _c_void_p],
     "iggt_write_special_tokens": [_c_void_p, _c_long, _c_long, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
                                   _c_int, _c_int, _c_void_p],
+    "iggt_packed_attn_ws_bytes": [_c_int] * 6,
+    "iggt_packed_attn_bf16": [_c_void_p, _c_long, _c_long] * 4 + [_c_void_p] * 2 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p,
+                                                                                                   _c_long, _c_void_p],
+    "iggt_packed_attn_f16": [_c_void_p, _c_long, _c_long] * 4 + [_c_void_p] * 2 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p,
+                                                                                                  _c_long, _c_void_p],
+    "iggt_paged_attn_ws_bytes": [_c_int] * 6,
+    "iggt_paged_attn_bf16": [_c_void_p, _c_long, _c_long] * 2 + [_c_void_p] * 4 + [_c_int] * 2 + [_c_void_p, _c_long, _c_int]
+                            + [_c_void_p] * 2 + [_c_int] * 7 + [_c_float, _c_int, _c_void_p, _c_long, _c_void_p],
+    "iggt_paged_attn_f16": [_c_void_p, _c_long, _c_long] * 2 + [_c_void_p] * 4 + [_c_int] * 2 + [_c_void_p, _c_long, _c_int]
+                           + [_c_void_p] * 2 + [_c_int] * 7 + [_c_float, _c_int, _c_void_p, _c_long, _c_void_p],
+    "iggt_append_pages_bf16": [_c_void_p, _c_long, _c_long] * 2 + [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 4 + [_c_void_p],
+    "iggt_append_pages_f16": [_c_void_p, _c_long, _c_long] * 2 + [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 4 + [_c_void_p],
+    "iggt_plan_pages": [_c_void_p, _c_long, _c_int, _c_int, _c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 4
+                       + [_c_int, _c_void_p],
 }
 
 
-_LONG_RETURN = {"iggt_flash_attn_static_ws_bytes", "iggt_flash_attn_static_est_ws_bytes", "iggt_linear_f32_ws_bytes"}
+_LONG_RETURN = {"iggt_flash_attn_static_ws_bytes", "iggt_flash_attn_static_est_ws_bytes", "iggt_linear_f32_ws_bytes",
+                "iggt_packed_attn_ws_bytes", "iggt_paged_attn_ws_bytes"}
 
 
 class HipExtensionError(RuntimeError):

@@ -1,0 +1,398 @@
+// Attention over a paged K/V cache held in 8 bits (e4m3 codes, one power-of-two scale per page and key head): few query rows per
+// request (single tokens, drafts), split over the keys; the fold of key ranges; and the dispatcher, which sends many rows per
+// request to the tile kernel of attention_packed.hip.
+//
+// Few rows: the bound is the read of the codes, 2 D bytes per key and key head.  A wave takes 64 keys at a time straight from
+// memory into registers -- no LDS, no barrier in the loop -- and the layouts are chosen so that every load is 16 bytes a lane and
+// nothing crosses lanes between load and matrix instruction (16 x 16 x 32, A = keys / channels, B = the up to 16 query rows):
+//   S^T:  row a of score tile t (t = 0 .. 3) is key 16 (a >> 2) + 4 t + (a & 3): lane group g = lane >> 4 then holds the scores of keys
+//         16 g .. 16 g + 15 of its query row, in order 4 t + r.  A lane's 16 bytes of K are channels 16 g .. 16 g + 15 of one key (two
+//         contraction steps); the query fragments use the same channel order.
+//   O^T:  the B operand of step u is the lane's own numerators 8 u .. 8 u + 7, so V^T must give lane (d, g) keys 16 g + 8 u ..: the cache
+//         keeps 16 keys of a channel side by side, one 16-byte load for both steps.
+// Scores are scaled by the page's 2^e in fp32; V is converted with its scale.  The next keys' K codes are loaded while this block's
+// softmax runs.  The four waves of a workgroup take every fourth block of its key range and are joined in LDS.
+#include "seq_attention.h"
+#include "../../include/iggt_hip.h"
+
+using namespace iggt_seq;
+
+namespace {
+
+template <int FMT>
+IGGT_DEVINL f32x4 mfma16h(bf16x8 a, bf16x8 b, f32x4 c) {
+    if (FMT == FMT_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// key range of split s: whole rounds of the four waves (256 keys)
+IGGT_DEVINL void key_blocks(int kend, int split, int splits, int& b0, int& b1) {
+    const int blocks = (kend + 63) >> 6, rounds = (blocks + 3) >> 2;
+    b0 = 4 * (int)((long)rounds * split / splits);
+    b1 = min(4 * (int)((long)rounds * (split + 1) / splits), blocks);
+}
+
+template <int D, int FMT>
+__global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnParams p) {
+    constexpr int NC = D / 64, NDT = D / 16;
+    constexpr float HALF = FMT == FMT_F16 ? 0.5f : 1.0f;   // fp16 holds half of V's values (a code at the top of its range is 2^16)
+    __shared__ float s_o[4][16][D + 4];
+    __shared__ float s_ml[4][16][2];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int npairs = p.B * p.Hkv;
+    const int pair = blockIdx.x % npairs, split = blockIdx.x / npairs;
+    const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+    const SeqSpan sp = seq_span<true>(p, b);
+    const int rows = sp.lq * p.G;
+    if (rows <= 0) return;
+    const int off = sp.lk - sp.lq;
+    const int kend = sp.lk;
+    const int first = p.causal ? max(min(sp.lk, off + 1), 0) : sp.lk;    // keys that every row sees
+    int b0, b1;
+    key_blocks(kend, split, p.splits, b0, b1);
+
+    const int rn = min(n, rows - 1), qi = rn / p.G, hq = h * p.G + rn - qi * p.G;
+    const int lim = p.causal ? max(min(sp.lk, off + qi + 1), 0) : sp.lk;
+    bf16x8 qf[NC][2];
+    {
+        const bf16_t* src = p.q + (long)(sp.q0 + qi) * p.q_rs + (long)hq * p.q_hs + 16 * g;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) qf[c][u] = *reinterpret_cast<const bf16x8*>(src + 64 * c + 8 * u);
+    }
+    f32x4 o[NDT];
+#pragma unroll
+    for (int i = 0; i < NDT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = M_INIT, l = 0.f;
+
+    const int pmask = (1 << p.page_shift) - 1;
+    const int a_sub = n >> 2, a_key = n & 3;
+    u32x4 kc[4][NC], vc[NDT];
+    int k_page, v_page;        // page of the lane's K rows / of its V keys in the block being loaded
+    auto pages = [&](int blk, int& kp, int& vp) {
+        kp = page_of(p, b, blk * 64 + a_sub * 16);
+        vp = page_of(p, b, blk * 64 + g * 16);
+    };
+    auto load_k = [&](int blk, int page) {
+        const uint8_t* src = p.k8 + (((((long)max(page, 0) * p.Hkv + h) << p.page_shift) + ((blk * 64 + a_sub * 16) & pmask) + a_key) * D) + 16 * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) kc[t][c] = *reinterpret_cast<const u32x4*>(src + (4 * t) * D + 64 * c);
+    };
+    auto load_v = [&](int blk, int page) {
+        const uint8_t* src = p.v8 + (((((long)max(page, 0) * p.Hkv + h) << p.page_shift) + ((blk * 64 + g * 16) & pmask)) * D) + n * 16;
+#pragma unroll
+        for (int i = 0; i < NDT; ++i) vc[i] = *reinterpret_cast<const u32x4*>(src + 256 * i);
+    };
+
+    int blk = b0 + wave;
+    if (blk < b1) {
+        pages(blk, k_page, v_page);
+        load_k(blk, k_page);
+    }
+    for (; blk < b1; blk += 4) {
+        const int vp = v_page;
+        load_v(blk, vp);
+        const long sidx = (long)max(vp, 0) * p.Hkv + h;
+        const float ks = scale_of(p.k_scale[sidx]) * p.scale_log2, vs = scale_of(p.v_scale[sidx]) * HALF;
+        const bool more = blk + 4 < b1;
+        if (more) pages(blk + 4, k_page, v_page);
+
+        f32x4 s[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                bf16x8 lo, hi;
+                cvt16<FMT>(kc[t][c], 1.0f, lo, hi);
+                s[t] = mfma16h<FMT>(lo, qf[c][0], s[t]);
+                s[t] = mfma16h<FMT>(hi, qf[c][1], s[t]);
+            }
+        }
+        if (more) load_k(blk + 4, k_page);
+
+        float e[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[4 * t + r] = s[t][r] * ks;
+        const int key0 = blk * 64 + g * 16;
+        const bool edge = blk * 64 + 64 > first || __any(vp < 0);
+        const int seen = vp < 0 ? 0 : lim - key0;       // of the lane's 16 keys, the first `seen` count for its row
+        if (edge) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j >= seen) e[j] = -INFINITY;
+        }
+        float mx = e[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, e[j]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < NDT; ++i) o[i] *= alpha;
+        }
+        const float ms = m - (FMT == FMT_F16 ? P_SHIFT_F16 : 0.f);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            e[j] = __builtin_amdgcn_exp2f(e[j] - ms);
+            l += e[j];
+        }
+        const bf16x8 p0 = pack8f<FMT>(e), p1 = pack8f<FMT>(e + 8);
+        bool bad = false;
+        if (edge) {
+            // codes 0x7f / 0xff are NaN (e4m3 has no infinity): behind the end they are whatever the page held, before it they belong
+            // to rows that see them
+            uint32_t nan = 0;
+#pragma unroll
+            for (int i = 0; i < NDT; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) nan |= ((vc[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            bad = __any(nan != 0);
+        }
+        if (!bad) {
+#pragma unroll
+            for (int i = 0; i < NDT; ++i) {
+                bf16x8 lo, hi;
+                cvt16<FMT>(vc[i], vs, lo, hi);
+                o[i] = mfma16h<FMT>(lo, p0, o[i]);
+                o[i] = mfma16h<FMT>(hi, p1, o[i]);
+            }
+        } else {
+            // the product runs on zeros in their place, and a second one of 0 / 1 codes with the mask finds the rows that see one
+            float one[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) one[j] = j < seen ? 1.f : 0.f;
+            const bf16x8 i0 = pack8f<FMT>(one), i1 = pack8f<FMT>(one + 8);
+#pragma unroll
+            for (int i = 0; i < NDT; ++i) {
+                u32x4 nan;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    nan[w] = ((((vc[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+                    vc[i][w] &= ~nan[w];
+                    nan[w] &= 0x38383838u;   // 1.0
+                }
+                bf16x8 lo, hi;
+                f32x4 cnt = {0.f, 0.f, 0.f, 0.f};
+                cvt16<FMT>(nan, 1.0f, lo, hi);
+                cnt = mfma16h<FMT>(lo, i0, cnt);
+                cnt = mfma16h<FMT>(hi, i1, cnt);
+                cvt16<FMT>(vc[i], vs, lo, hi);
+                o[i] = mfma16h<FMT>(lo, p0, o[i]);
+                o[i] = mfma16h<FMT>(hi, p1, o[i]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (cnt[r] > 0.f) o[i][r] = __builtin_nanf("");
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+
+    // ---- join the four waves
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) {
+        s_ml[wave][n][0] = m;
+        s_ml[wave][n][1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < NDT; ++i) *reinterpret_cast<f32x4*>(&s_o[wave][n][16 * i + 4 * g]) = o[i];
+    __syncthreads();
+    constexpr int LPR = D / 4;   // lanes of a row, four channels each
+    for (int r = tid / LPR; r < rows; r += 256 / LPR) {
+        const int d = (tid % LPR) * 4;
+        float mm = s_ml[0][r][0];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, s_ml[w][r][0]);
+        float ll = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (s_ml[w][r][1] == 0.f) continue;
+            const float f = __builtin_amdgcn_exp2f(s_ml[w][r][0] - mm);
+            ll += s_ml[w][r][1] * f;
+            acc += *reinterpret_cast<const f32x4*>(&s_o[w][r][d]) * f;
+        }
+        const int i = r / p.G, hr = h * p.G + r - i * p.G;
+        if (p.splits > 1) {
+            const long at = (((long)split * p.B + b) * p.max_q + i) * p.Hq + hr;
+            if (d == 0) {
+                p.part_ml[2 * at] = mm;
+                p.part_ml[2 * at + 1] = ll;
+            }
+            if (ll != 0.f) *reinterpret_cast<f32x4*>(p.part_o + at * D + d) = acc;
+        } else {
+            const float inv = ll == 0.f ? 0.f : (1.0f / HALF) / ll;
+            u32x2 w;
+            w[0] = pack_h2<FMT, false>(acc[0] * inv, acc[1] * inv);
+            w[1] = pack_h2<FMT, false>(acc[2] * inv, acc[3] * inv);
+            *reinterpret_cast<u32x2*>(p.o + (long)(sp.q0 + i) * p.o_rs + (long)hr * p.o_hs + d) = w;
+        }
+    }
+}
+
+// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the key ranges: one wave per row, D / 4 lanes of four channels each, the
+// remaining lane groups (4 of D = 64, 2 of D = 128) take every 4th / 2nd range.
+template <int D, int FMT, bool PAGED>
+__global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams p) {
+    constexpr int LPR = D / 4, NG = 64 / LPR;
+    constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
+    const int lane = threadIdx.x & 63, gr = lane / LPR, d = (lane % LPR) * 4;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);    // ((b, token), head)
+    const long per = (long)p.max_q * p.Hq;
+    const int b = (int)(row / per);
+    if (b >= p.B) return;
+    const int i = (int)((row - b * per) / p.Hq), hq = (int)(row % p.Hq);
+    const SeqSpan sp = seq_span<PAGED>(p, b);
+    if (i >= sp.lq) return;
+    const long step = (long)p.B * per;
+    float mm = M_INIT;
+    for (int s = gr; s < p.splits; s += NG) mm = fmaxf(mm, p.part_ml[2 * (s * step + row)]);
+#pragma unroll
+    for (int x = LPR; x < 64; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
+    float ll = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = gr; s < p.splits; s += NG) {
+        const long at = s * step + row;
+        const float lp = p.part_ml[2 * at + 1];
+        if (lp == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - mm);
+        ll += lp * f;
+        acc += *reinterpret_cast<const f32x4*>(p.part_o + at * D + d) * f;
+    }
+#pragma unroll
+    for (int x = LPR; x < 64; x *= 2) {
+        ll += __shfl_xor(ll, x, 64);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], x, 64);
+    }
+    if (gr == 0) {
+        const float inv = ll == 0.f ? 0.f : (1.0f / HALF) / ll;
+        u32x2 w;
+        w[0] = pack_h2<FMT, false>(acc[0] * inv, acc[1] * inv);
+        w[1] = pack_h2<FMT, false>(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<u32x2*>(p.o + (long)(sp.q0 + i) * p.o_rs + (long)hq * p.o_hs + d) = w;
+    }
+}
+
+template <int D>
+int launch_fold(const SeqAttnParams& p, int fmt, bool paged, hipStream_t stream) {
+    const long rows = (long)p.B * p.max_q * p.Hq, n = (rows + 3) / 4;
+    if (n >= (1L << 31)) return -4;
+    const dim3 grid((unsigned)n), block(256);
+    if (fmt == FMT_F16) {
+        if (paged) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_F16, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_F16, false>), grid, block, 0, stream, p);
+    } else {
+        if (paged) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_BF16, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_BF16, false>), grid, block, 0, stream, p);
+    }
+    IGGT_CHECK_LAUNCH();
+    return 0;
+}
+
+template <int D>
+int launch_rows(const SeqAttnParams& p, int fmt, hipStream_t stream) {
+    const long n = (long)p.splits * p.B * p.Hkv;
+    if (n >= (1L << 31)) return -4;
+    const dim3 grid((unsigned)n), block(256);
+    if (fmt == FMT_F16) hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_F16>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_BF16>), grid, block, 0, stream, p);
+    IGGT_CHECK_LAUNCH();
+    return 0;
+}
+
+// Up to 16 rows per (request, key head): the row kernel, its key ranges multiples of 256 keys, as many as give the chip 4
+// workgroups per CU.
+bool few_rows(long max_q, int G) { return max_q * G <= 16; }
+SeqPlan paged_plan(int B, long max_q, long max_len, int Hkv, int G, int D) {
+    if (!few_rows(max_q, G)) return iggt_seq_tile_plan(B, max_q, max_len, Hkv, G, D);
+    const long pairs = (long)B * Hkv, most = (max_len + 255) / 256;
+    long s = (1024 + pairs - 1) / pairs;
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+    SeqPlan plan = {(int)s, false};
+    return plan;
+}
+
+int page_shift_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
+
+}  // namespace
+
+int iggt_launch_seq_fold(const SeqAttnParams& p, int D, int fmt, bool paged, hipStream_t stream) {
+    return D == 64 ? launch_fold<64>(p, fmt, paged, stream) : launch_fold<128>(p, fmt, paged, stream);
+}
+
+static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o, long o_rs, long o_hs, const void* k_codes,
+                          const void* k_scale, const void* v_codes, const void* v_scale, int num_pages, int page,
+                          const int* tables, long table_stride, int table_width, const int* lens, const int* cu_q, int B, int Tq,
+                          int max_q, int max_len, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                          void* stream) {
+    const int shift = page_shift_of(page);
+    if (B < 0 || Tq < 0 || max_q < 0 || max_len < 0 || num_pages < 0 || table_width < 0 || shift < 0) return -1;
+    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
+    if ((long)table_width * page >= (1L << 31) || (cu_q == nullptr && max_q > 1)) return -1;
+    if ((q_rs | q_hs) % 8 || (o_rs | o_hs) % 4 || (uintptr_t)q % 16 || (uintptr_t)o % 8) return -2;
+    if (((uintptr_t)k_codes | (uintptr_t)v_codes) % 16) return -2;
+    if (!(scale > 0.f)) return -3;
+    if (B == 0 || Tq == 0 || max_q == 0) return 0;
+    SeqAttnParams p = {};
+    p.q = (const bf16_t*)q; p.o = (bf16_t*)o;
+    p.q_rs = q_rs; p.q_hs = q_hs; p.o_rs = o_rs; p.o_hs = o_hs;
+    p.k8 = (const uint8_t*)k_codes; p.v8 = (const uint8_t*)v_codes;
+    p.k_scale = (const uint8_t*)k_scale; p.v_scale = (const uint8_t*)v_scale;
+    p.tables = tables; p.table_stride = table_stride; p.table_width = num_pages > 0 ? table_width : 0; p.lens = lens;
+    p.num_pages = num_pages; p.page_shift = shift; p.cu_q = cu_q;
+    p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.Tq = Tq; p.max_q = max_q; p.causal = causal != 0;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    const SeqPlan plan = paged_plan(B, max_q, max_len, Hkv, p.G, D);
+    p.splits = plan.splits;
+    if (p.splits > 1) {
+        const long n = (long)p.splits * B * max_q * Hq;
+        if (ws == nullptr || ws_len < n * (D + 2) * 4 || (uintptr_t)ws % 16) return -5;
+        p.part_o = (float*)ws;
+        p.part_ml = p.part_o + n * D;
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    int rc;
+    if (few_rows(max_q, p.G)) rc = D == 64 ? launch_rows<64>(p, fmt, st) : launch_rows<128>(p, fmt, st);
+    else rc = iggt_launch_seq_tiles(p, D, fmt, true, plan.small, st);
+    if (rc || p.splits == 1) return rc;
+    return iggt_launch_seq_fold(p, D, fmt, true, st);
+}
+
+extern "C" {
+long iggt_paged_attn_ws_bytes(int B, int max_q, int max_len, int Hq, int Hkv, int D) {
+    if (B <= 0 || max_q <= 0 || max_len < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return 0;
+    const SeqPlan plan = paged_plan(B, max_q, max_len, Hkv, Hq / Hkv, D);
+    return plan.splits > 1 ? (long)plan.splits * B * max_q * Hq * (D + 2) * 4 : 0;
+}
+int iggt_paged_attn_bf16(const void* q, long q_rs, long q_hs, void* o, long o_rs, long o_hs, const void* k_codes,
+                         const void* k_scale, const void* v_codes, const void* v_scale, int num_pages, int page,
+                         const int* tables, long table_stride, int table_width, const int* lens, const int* cu_q, int B, int Tq,
+                         int max_q, int max_len, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                         void* stream) {
+    return paged_attn_h16(FMT_BF16, q, q_rs, q_hs, o, o_rs, o_hs, k_codes, k_scale, v_codes, v_scale, num_pages, page, tables,
+                          table_stride, table_width, lens, cu_q, B, Tq, max_q, max_len, Hq, Hkv, D, scale, causal, ws, ws_len, stream);
+}
+int iggt_paged_attn_f16(const void* q, long q_rs, long q_hs, void* o, long o_rs, long o_hs, const void* k_codes,
+                        const void* k_scale, const void* v_codes, const void* v_scale, int num_pages, int page,
+                        const int* tables, long table_stride, int table_width, const int* lens, const int* cu_q, int B, int Tq,
+                        int max_q, int max_len, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                        void* stream) {
+    return paged_attn_h16(FMT_F16, q, q_rs, q_hs, o, o_rs, o_hs, k_codes, k_scale, v_codes, v_scale, num_pages, page, tables,
+                          table_stride, table_width, lens, cu_q, B, Tq, max_q, max_len, Hq, Hkv, D, scale, causal, ws, ws_len, stream);
+}
+}

@@ -493,6 +493,67 @@ int iggt_hdbscan_nearest_foreign_f32(const float* x, const float* core2, const i
 int iggt_hdbscan_labels_from_mst(const int* eu, const int* ev, const float* ew, long n_points, int min_cluster_size,
                                  double cluster_selection_epsilon, int allow_single_cluster, int* labels);
 
+/* ---- attention over packed sequences, and over a paged 8-bit K/V cache (no counterpart in the reference, whose
+ * F.scaled_dot_product_attention, iggt/layers/attention.py:60-66, sees equal-length batches whole) -------------------
+ *
+ *   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - m_i) / l_i  over the keys j of i's own sequence, with
+ *   j <= i + Lk - Lq if causal (the last row sees the last key).  A row that sees no key is 0.
+ *
+ * q / o: 16-bit [Tq][Hq][D], k / v: 16-bit [Tk][Hkv][D], row and head strides in elements (multiples of 8, o: of 4), channels
+ * contiguous, q / k / v 16-byte and o 8-byte aligned; D = 64 | 128; query head h reads key head h / (Hq / Hkv).  Sequence b is
+ * rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] .. cu_k[b + 1] (int32 on the device, clamped to the tensors); max_q / max_k bound the
+ * lengths from above (rows past max_q of a sequence are not computed; max_k only chooses the number of key ranges).  Rows of o
+ * outside the sequences are left as they are.  scale > 0.  ws: scratch of at least ..._ws_bytes (0: none needed), 16-byte
+ * aligned, for this call alone while it runs. */
+long iggt_packed_attn_ws_bytes(int B, int max_q, int max_k, int Hq, int Hkv, int D);
+int iggt_packed_attn_bf16(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs,
+                          long v_hs, void* o, long o_rs, long o_hs, const int* cu_q, const int* cu_k, int B, int Tq, int Tk,
+                          int max_q, int max_k, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                          void* stream);
+int iggt_packed_attn_f16(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs,
+                         long v_hs, void* o, long o_rs, long o_hs, const int* cu_q, const int* cu_k, int B, int Tq, int Tk,
+                         int max_q, int max_k, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                         void* stream);
+
+/* The cache: pages of `page` tokens (16 | 32 | 64 | 128).  K codes e4m3 [num_pages][Hkv][page][D], V codes e4m3
+ * [num_pages][Hkv][page / 16][D][16] (16 tokens of a channel side by side); one scale per page and key head for each,
+ * 2^(byte - 127), [num_pages][Hkv].  Request b's token t is place t % page of page tables[b][t / page] (tables int32
+ * [B][table_stride], table_width entries valid).  All of codes 16-byte aligned.
+ *
+ * iggt_paged_attn_*: the formula above with k, v = code * 2^(byte - 127); request b holds lens[b] tokens (int32 on the device,
+ * clamped to [0, table_width * page]; max_len bounds them and chooses the number of key ranges).  cu_q == NULL: request b's one
+ * query row is row b (max_q <= 1).  Tokens on a page that does not exist (entry outside [0, num_pages)) count as not there. */
+long iggt_paged_attn_ws_bytes(int B, int max_q, int max_len, int Hq, int Hkv, int D);
+int iggt_paged_attn_bf16(const void* q, long q_rs, long q_hs, void* o, long o_rs, long o_hs, const void* k_codes,
+                         const void* k_scale, const void* v_codes, const void* v_scale, int num_pages, int page,
+                         const int* tables, long table_stride, int table_width, const int* lens, const int* cu_q, int B, int Tq,
+                         int max_q, int max_len, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                         void* stream);
+int iggt_paged_attn_f16(const void* q, long q_rs, long q_hs, void* o, long o_rs, long o_hs, const void* k_codes,
+                        const void* k_scale, const void* v_codes, const void* v_scale, int num_pages, int page,
+                        const int* tables, long table_stride, int table_width, const int* lens, const int* cu_q, int B, int Tq,
+                        int max_q, int max_len, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
+                        void* stream);
+/* Writes tokens 0 .. T - 1 (k / v like above) at slots[t] = page id * page + place (int32; outside the cache: token skipped).
+ * Tokens of a page come as one run of consecutive slots per call, in order; places below the run's first are held tokens, those
+ * above its last are not.  Scale of a page: the least 2^e with amax <= 448 * 2^e over the finite values, never below the one of
+ * the tokens it holds (their codes are rewritten when it grows).  Infinities are written as the largest value, NaN as NaN. */
+int iggt_append_pages_bf16(const void* k, long k_rs, long k_hs, const void* v, long v_rs, long v_hs, const int* slots, int tokens,
+                           void* k_codes, void* k_scale, void* v_codes, void* v_scale, int num_pages, int page, int Hkv, int D,
+                           void* stream);
+int iggt_append_pages_f16(const void* k, long k_rs, long k_hs, const void* v, long v_rs, long v_hs, const int* slots, int tokens,
+                          void* k_codes, void* k_scale, void* v_codes, void* v_scale, int num_pages, int page, int Hkv, int D,
+                          void* stream);
+/* One step of the page tables (all int32 on the device): requests (<= 8192) hold lens[b] tokens and are to hold new_lens[b] (both
+ * clamped to [0, table_width * page]).  Growing requests take pages off the ring of free pages (ring[(counters[0] + i) % num_pages],
+ * i < counters[1]), shrinking ones put theirs behind its tail, both in request order; tables and ring are updated in place.
+ *   slots [num_slots]: slot of every added token in request order, -1 behind the last;  starts [requests + 1]: its prefix sums
+ *   next_lens [requests], next_counters [3]: lengths, (head, free pages) after the step, and the number of pages that were missing
+ * With pages missing, or -1 (num_slots too short), no request grows in this step.  Outputs do not overlap the inputs. */
+int iggt_plan_pages(int* tables, long table_stride, int requests, int table_width, int* ring, int num_pages, const int* counters,
+                    const int* lens, const int* new_lens, int page, int* starts, int* next_lens, int* next_counters, int* slots,
+                    int num_slots, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
