@@ -23,21 +23,52 @@ namespace {
 
 constexpr float DEFER_THR = 4.0f;
 
-template <int D, int QB, int FMT, bool PAGED>
+// Order of the work items.  Longest first, so that the last ones to start are short: under a causal mask the last query tiles, else
+// the sequences by their number of keys (up to 64 of them: ranked here, one lane each).  Key heads innermost: consecutive workgroups
+// go to the XCDs in turn, so one head's tiles share an L2.  Where (sequence, head) pairs are a multiple of 8 but heads are not, an
+// XCD would keep one sequence for good: the pairs move on by one every 16th of the tiles.
+template <bool PAGED>
+IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt, int& b, int& h) {
+    int w = blockIdx.x;
+    if (p.causal || p.B == 1 || p.B > 64) {
+        const int npairs = p.B * p.Hkv;
+        int pair = w % npairs;
+        w /= npairs;
+        split = w % p.splits;
+        const int at = w / p.splits;
+        qt = p.qtiles - 1 - at;
+        pair = (pair + at / ((p.qtiles >> 4) + 1)) % npairs;
+        b = pair / p.Hkv;
+        h = pair - b * p.Hkv;
+    } else {
+        h = w % p.Hkv;
+        w /= p.Hkv;
+        split = w % p.splits;
+        w /= p.splits;
+        qt = w % p.qtiles;
+        const int place = w / p.qtiles;
+        const int lk = lane < p.B ? seq_span<PAGED>(p, lane).lk : -1;
+        int rank = 0;
+        for (int i = 0; i < p.B; ++i) {
+            const int other = __builtin_amdgcn_readlane(lk, i);
+            rank += (other > lk || (other == lk && i < lane)) ? 1 : 0;
+        }
+        const unsigned long long mine = __ballot(lane < p.B && rank == place);
+        b = (int)__builtin_ctzll(mine);
+    }
+}
+
+template <int D, int QB, int KVM, int FMT, bool PAGED>
 __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnParams p) {
-    constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, BUF = 2 * K_BYTES, NKC = D / 16, NDH = D / 32, BM = 128 * QB;
+    constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, TILE = 2 * K_BYTES, BUF = KVM * TILE, NKC = D / 16, NDH = D / 32, BM = 128 * QB;
     constexpr int SLOTS = ROWB / 16;   // 16-byte slots of a K row
     __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int frow = lane & 31, fhalf = lane >> 5;
 
-    // work order: last (under a causal mask longest) query tiles first; (sequence, key head) pairs innermost, so that consecutive
-    // workgroups -- one per XCD in turn -- take different pairs, and with a multiple of 8 pairs every pair stays on one XCD's L2
-    const int npairs = p.B * p.Hkv;
-    const int pair = blockIdx.x % npairs, rest = blockIdx.x / npairs;
-    const int split = rest % p.splits, qt = p.qtiles - 1 - rest / p.splits;
-    const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+    int split, qt, b, h;
+    work_item<PAGED>(p, lane, split, qt, b, h);
     const SeqSpan sp = seq_span<PAGED>(p, b);
     const long rows = (long)sp.lq * p.G;
     const long row0 = (long)qt * BM;
@@ -48,7 +79,8 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     };
     const int kend = limit_of(min(row0 + BM, rows) - 1);
     const int ktiles = (kend + 63) >> 6;
-    const int t0 = (int)((long)ktiles * split / p.splits), t1 = (int)((long)ktiles * (split + 1) / p.splits);
+    const int mtiles = (ktiles + KVM - 1) / KVM;                    // macro tiles of 64 KVM keys: one barrier each
+    const int t0 = (int)((long)mtiles * split / p.splits), t1 = (int)((long)mtiles * (split + 1) / p.splits);
 
     const int wg_first = limit_of(row0);   // keys every row of the tile sees
     const long wrow = row0 + wave * (32 * QB);
@@ -76,30 +108,45 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     constexpr int CPW = K_BYTES / 1024 / 4;     // chunks per wave
     const bf16_t* kb_ptr = nullptr;
     const bf16_t* vb_ptr = nullptr;
+    int drow[CPW], kcol[CPW], vcol[CPW];        // row and swizzled byte column of the lane's piece in each of its chunks
+    uint32_t koffs[CPW], voffs[CPW];            // their byte offsets within a tile (host: a tile spans less than 2^32)
     if constexpr (!PAGED) {
         kb_ptr = p.k + (long)sp.k0 * p.k_rs + (long)h * p.k_hs;
         vb_ptr = p.v + (long)sp.k0 * p.v_rs + (long)h * p.v_hs;
-    }
-    auto dma = [&](int t, int buf) {
-        char* sK = smem + buf * BUF;
-        char* sV = sK + K_BYTES;
-        const bool ragged = (t + 1) * 64 > sp.lk;
 #pragma unroll
         for (int i = 0; i < CPW; ++i) {
-            const int chunk = wave * CPW + i;
-            const int r = chunk * RPC + lane / SLOTS, pos = lane % SLOTS;
-            int kpiece, vpiece;
-            if constexpr (D == 64) {
-                kpiece = pos ^ ((r >> 1) & 7);
-                vpiece = (((pos >> 1) ^ (r & 2)) << 1) | (pos & 1);
+            const int r = (wave * CPW + i) * RPC + lane / SLOTS, pos = lane % SLOTS;
+            drow[i] = r;
+            kcol[i] = (D == 64 ? pos ^ ((r >> 1) & 7) : pos ^ (r & 15)) * 16;
+            vcol[i] = (D == 64 ? (((pos >> 1) ^ (r & 2)) << 1) | (pos & 1) : (((pos >> 1) ^ ((r & 3) << 1)) << 1) | (pos & 1)) * 16;
+            koffs[i] = (uint32_t)r * (uint32_t)(2 * p.k_rs) + kcol[i];
+            voffs[i] = (uint32_t)r * (uint32_t)(2 * p.v_rs) + vcol[i];
+        }
+    }
+    auto dma = [&](int mt, int buf) {
+#pragma unroll
+        for (int sub = 0; sub < KVM; ++sub) {
+            const int t = mt * KVM + sub;
+            if (KVM > 1 && t >= ktiles) break;
+            char* sK = smem + buf * BUF + sub * TILE;
+            char* sV = sK + K_BYTES;
+            const char* kt = reinterpret_cast<const char*>(kb_ptr + (long)t * 64 * p.k_rs);
+            const char* vt = reinterpret_cast<const char*>(vb_ptr + (long)t * 64 * p.v_rs);
+            const int left = sp.lk - 1 - t * 64;
+            if (left < 63) {
+#pragma unroll
+                for (int i = 0; i < CPW; ++i) {
+                    const uint32_t r = min(drow[i], left);
+                    __builtin_amdgcn_global_load_lds((gptr_t*)(kt + (r * (uint32_t)(2 * p.k_rs) + kcol[i])), (lptr_t*)(sK + (wave * CPW + i) * 1024), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((gptr_t*)(vt + (r * (uint32_t)(2 * p.v_rs) + vcol[i])), (lptr_t*)(sV + (wave * CPW + i) * 1024), 16, 0, 0);
+                }
             } else {
-                kpiece = pos ^ (r & 15);
-                vpiece = (((pos >> 1) ^ ((r & 3) << 1)) << 1) | (pos & 1);
+#pragma unroll
+                for (int i = 0; i < CPW; ++i) {
+                    __builtin_amdgcn_global_load_lds((gptr_t*)(kt + koffs[i]), (lptr_t*)(sK + (wave * CPW + i) * 1024), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((gptr_t*)(vt + voffs[i]), (lptr_t*)(sV + (wave * CPW + i) * 1024), 16, 0, 0);
+                }
             }
-            int key = t * 64 + r;
-            if (ragged) key = min(key, sp.lk - 1);
-            __builtin_amdgcn_global_load_lds((gptr_t*)(kb_ptr + (long)key * p.k_rs + kpiece * 8), (lptr_t*)(sK + chunk * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr_t*)(vb_ptr + (long)key * p.v_rs + vpiece * 8), (lptr_t*)(sV + chunk * 1024), 16, 0, 0);
         }
     };
     // 8-bit: codes go through registers (16 bytes each), are converted and written as 16-bit tiles: K rows like above, V transposed
@@ -109,40 +156,40 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     constexpr int PPT = D / 64;   // 16-byte pieces of K (and of V) per thread
     constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
     u32x4 k8r[PPT], v8r[PPT];
-    float kscl[PPT], vscl[PPT];
+    uint32_t kbyte[PPT], vbyte[PPT];
     uint32_t have_next = 0xf, have = 0xf;       // which 16-key groups of the tile have a page
+    // a wave's piece i lies in one 16-key group: one table entry, loaded a tile ahead (lane l: group l & 3), serves its K and its V
+    const int psub = D == 64 ? wave : wave >> 1;
+    int pid = -1;
+    auto look_up = [&](int t) { pid = page_of(p, b, t * 64 + (lane & 3) * 16); };
     auto fetch = [&](int t) {
-        const int base = t * 64;
+        have_next = (uint32_t)__ballot(pid >= 0) & 0xfu;
+        const int pmask = (1 << p.page_shift) - 1;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
-            const int c = tid + 256 * i;
-            const int key = c / (D / 16), piece = c % (D / 16);
-            const int pk = max(page_of(p, b, base + key), 0);
-            const long kp = (long)pk * p.Hkv + h;
-            k8r[i] = *reinterpret_cast<const u32x4*>(p.k8 + ((kp << p.page_shift) + ((base + key) & ((1 << p.page_shift) - 1))) * D + piece * 16);
-            kscl[i] = scale_of(p.k_scale[kp]) * HALF;
-            const int sub = c / D, d = c % D;
-            const int pv = max(page_of(p, b, base + sub * 16), 0);
-            const long vp = (long)pv * p.Hkv + h;
-            v8r[i] = *reinterpret_cast<const u32x4*>(p.v8 + ((vp << p.page_shift) + ((base + sub * 16) & ((1 << p.page_shift) - 1))) * D + d * 16);
-            vscl[i] = scale_of(p.v_scale[vp]) * HALF;
+            const int sub = psub + 2 * i;
+            const long head = (long)max(__builtin_amdgcn_readlane(pid, sub), 0) * p.Hkv + h;
+            const long at = ((head << p.page_shift) + ((t * 64 + sub * 16) & pmask)) * D;      // of the group's K rows, and of its V
+            const int in = D == 64 ? lane * 16 : ((wave & 1) * 64 + lane) * 16;
+            k8r[i] = *reinterpret_cast<const u32x4*>(p.k8 + at + in);
+            v8r[i] = *reinterpret_cast<const u32x4*>(p.v8 + at + in);
+            kbyte[i] = p.k_scale[head];
+            vbyte[i] = p.v_scale[head];
         }
-        have_next = (uint32_t)__ballot(page_of(p, b, base + (lane & 3) * 16) >= 0) & 0xfu;
     };
     auto stage = [&](int buf) {
         char* sK = smem + buf * BUF;
         char* sV = sK + K_BYTES;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
-            const int c = tid + 256 * i;
-            const int key = c / (D / 16), piece = c % (D / 16);
+            const int sub = psub + 2 * i, in = D == 64 ? lane : (wave & 1) * 64 + lane;     // 16-byte piece of the group
+            const int key = sub * 16 + in / (D / 16), piece = in % (D / 16), d = in;
             bf16x8 lo, hi;
-            cvt16<FMT>(k8r[i], kscl[i], lo, hi);
+            cvt16<FMT>(k8r[i], scale_of(kbyte[i]) * HALF, lo, hi);
             const int sw = D == 64 ? (key >> 1) & 7 : key & 15;
             *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece) ^ sw) * 16) = lo;
             *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece + 1) ^ sw) * 16) = hi;
-            const int sub = c / D, d = c % D;
-            cvt16<FMT>(v8r[i], vscl[i], lo, hi);
+            cvt16<FMT>(v8r[i], scale_of(vbyte[i]) * HALF, lo, hi);
             const u32x4 a = __builtin_bit_cast(u32x4, lo), z = __builtin_bit_cast(u32x4, hi);
             const u32x4 x = {a[0], a[1], z[0], z[1]}, y = {a[2], a[3], z[2], z[3]};
             *reinterpret_cast<u32x4*>(sV + swz_off(d, 2 * sub)) = x;
@@ -301,27 +348,47 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         __syncthreads();
     };
 
+    // keeps the packed numerators of the first query block where they are formed, beside the second block's score products
+    auto pin = [&](bf16x8 (&pf)[2][2]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u32x4 w = __builtin_bit_cast(u32x4, pf[i >> 1][i & 1]);
+            asm volatile("" : "+v"(w));
+            pf[i >> 1][i & 1] = __builtin_bit_cast(bf16x8, w);
+        }
+    };
+
     if (t0 < t1) {
         if constexpr (PAGED) {
+            look_up(t0);
             fetch(t0);
+            if (t0 + 1 < t1) look_up(t0 + 1);
             stage(t0 & 1);
         } else {
             dma(t0, t0 & 1);
         }
         __syncthreads();   // (drains the DMA as well)
-        for (int t = t0; t < t1; ++t) {
-            if (t + 1 < t1) {
-                if constexpr (PAGED) fetch(t + 1);
-                else dma(t + 1, (t + 1) & 1);
+        for (int mt = t0; mt < t1; ++mt) {
+            if (mt + 1 < t1) {
+                if constexpr (PAGED) {
+                    fetch(mt + 1);
+                    if (mt + 2 < t1) look_up(mt + 2);
+                } else {
+                    dma(mt + 1, (mt + 1) & 1);
+                }
             }
-            char* sK = smem + (t & 1) * BUF;
-            char* sV = sK + K_BYTES;
-            if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
-                bool bad = false;
-                for (int i = tid * 16; i < K_BYTES; i += 4096) bad = bad || nonfinite8<FMT>(*reinterpret_cast<const bf16x8*>(sV + i));
-                if (__syncthreads_or(bad)) absorb_nonfinite(sK, sV, t);
-            }
-            if (t * 64 < w_last) {
+#pragma unroll
+            for (int sub = 0; sub < KVM; ++sub) {
+                const int t = mt * KVM + sub;
+                if (KVM > 1 && t >= ktiles) break;
+                char* sK = smem + (mt & 1) * BUF + sub * TILE;
+                char* sV = sK + K_BYTES;
+                if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
+                    bool bad = false;
+                    for (int i = tid * 16; i < K_BYTES; i += 4096) bad = bad || nonfinite8<FMT>(*reinterpret_cast<const bf16x8*>(sV + i));
+                    if (__syncthreads_or(bad)) absorb_nonfinite(sK, sV, t);
+                }
+                if (t * 64 >= w_last) continue;
                 const bool edge = (t + 1) * 64 > w_first || (PAGED && have != 0xf);
                 f32x16 s0[2], s1[2];
                 bf16x8 pf0[2][2], pf1[2][2];
@@ -331,6 +398,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
                 if constexpr (QB == 2) qk(sK, 1, s1);
                 exp_pack(0, s0, pf0);
                 if constexpr (QB == 2) {
+                    pin(pf0);
                     if (edge) mask(t, 1, s1);
                     update_max(1, s1);
                 }
@@ -341,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
                 }
             }
             if constexpr (PAGED) {
-                if (t + 1 < t1) stage((t + 1) & 1);
+                if (mt + 1 < t1) stage((mt + 1) & 1);
             }
             __syncthreads();
         }
@@ -385,21 +453,22 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     }
 }
 
-template <int D, int QB, int FMT, bool PAGED>
+template <int D, int QB, int KVM, int FMT, bool PAGED>
 int launch(const SeqAttnParams& p_in, hipStream_t stream) {
     SeqAttnParams p = p_in;
     p.qtiles = (int)(((long)p.max_q * p.G + 128 * QB - 1) / (128 * QB));
     const long n = (long)p.qtiles * p.splits * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
-    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, FMT, PAGED>), dim3((unsigned)n), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, KVM, FMT, PAGED>), dim3((unsigned)n), dim3(256), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
 }
 
 template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
-    if (D == 128) return launch<128, 1, FMT, PAGED>(p, stream);
-    return small ? launch<64, 1, FMT, PAGED>(p, stream) : launch<64, 2, FMT, PAGED>(p, stream);
+    if (D == 128) return launch<128, 1, 1, FMT, PAGED>(p, stream);
+    constexpr int KVM = PAGED ? 1 : 2;
+    return small ? launch<64, 1, KVM, FMT, PAGED>(p, stream) : launch<64, 2, KVM, FMT, PAGED>(p, stream);
 }
 
 }  // namespace
@@ -410,7 +479,7 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
 }
 
 SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D) {
-    SeqPlan plan;
+    SeqPlan plan = {};
     const long rows = max_q * G, pairs = (long)B * Hkv, slots = 512;   // two workgroups on each of 256 CUs
     plan.small = D == 64 && (rows <= 128 || pairs * ((rows + 255) / 256) < slots);
     const int bm = (D == 128 || plan.small) ? 128 : 256;
@@ -434,6 +503,7 @@ static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const v
     if (B < 0 || Tq < 0 || Tk < 0 || max_q < 0 || max_k < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
     if ((q_rs | q_hs | k_rs | k_hs | v_rs | v_hs) % 8 || (o_rs | o_hs) % 4) return -2;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || (uintptr_t)o % 8) return -2;
+    if (k_rs < 0 || v_rs < 0 || k_rs >= (1L << 24) || v_rs >= (1L << 24)) return -2;   // 64 rows in 32-bit byte offsets
     if (!(scale > 0.f)) return -3;
     if (B == 0 || Tq == 0 || max_q == 0) return 0;
     SeqAttnParams p = {};

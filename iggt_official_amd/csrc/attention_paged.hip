@@ -26,13 +26,6 @@ IGGT_DEVINL f32x4 mfma16h(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// key range of split s: whole rounds of the four waves (256 keys)
-IGGT_DEVINL void key_blocks(int kend, int split, int splits, int& b0, int& b1) {
-    const int blocks = (kend + 63) >> 6, rounds = (blocks + 3) >> 2;
-    b0 = 4 * (int)((long)rounds * split / splits);
-    b1 = min(4 * (int)((long)rounds * (split + 1) / splits), blocks);
-}
-
 template <int D, int FMT>
 __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnParams p) {
     constexpr int NC = D / 64, NDT = D / 16;
@@ -50,8 +43,9 @@ __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnPara
     const int off = sp.lk - sp.lq;
     const int kend = sp.lk;
     const int first = p.causal ? max(min(sp.lk, off + 1), 0) : sp.lk;    // keys that every row sees
-    int b0, b1;
-    key_blocks(kend, split, p.splits, b0, b1);
+    // key range of the work item: whole rounds of the four waves (256 keys), of the same length for every request
+    const int b0 = split * p.range_blocks;
+    const int b1 = split == p.splits - 1 ? (kend + 63) >> 6 : min(b0 + p.range_blocks, (kend + 63) >> 6);   // (max_len may be too small)
 
     const int rn = min(n, rows - 1), qi = rn / p.G, hq = h * p.G + rn - qi * p.G;
     const int lim = p.causal ? max(min(sp.lk, off + qi + 1), 0) : sp.lk;
@@ -242,43 +236,67 @@ __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnPara
     }
 }
 
-// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the key ranges: one wave per row, D / 4 lanes of four channels each, the
-// remaining lane groups (4 of D = 64, 2 of D = 128) take every 4th / 2nd range.
-template <int D, int FMT, bool PAGED>
+// o = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(m_s - M), over up to FOLD_MAX key ranges.  W waves share a row (four where there are few
+// rows: the loads of a row are then a chain of a few); a wave's lanes hold the weights of all ranges, D / 4 lanes take four channels
+// of one range each.
+template <int D, int FMT, bool PAGED, int W>
 __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams p) {
     constexpr int LPR = D / 4, NG = 64 / LPR;
     constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
-    const int lane = threadIdx.x & 63, gr = lane / LPR, d = (lane % LPR) * 4;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);    // ((b, token), head)
+    __shared__ f32x4 s_acc[4][LPR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, gr = lane / LPR, d = (lane % LPR) * 4;
+    const long row = (long)blockIdx.x * (4 / W) + wave / W;    // ((b, token), head)
     const long per = (long)p.max_q * p.Hq;
     const int b = (int)(row / per);
-    if (b >= p.B) return;
+    SeqSpan sp = {0, 0, 0, 0};
+    if (b < p.B) sp = seq_span<PAGED>(p, b);
     const int i = (int)((row - b * per) / p.Hq), hq = (int)(row % p.Hq);
-    const SeqSpan sp = seq_span<PAGED>(p, b);
-    if (i >= sp.lq) return;
+    const bool live = b < p.B && i < sp.lq;
     const long step = (long)p.B * per;
-    float mm = M_INIT;
-    for (int s = gr; s < p.splits; s += NG) mm = fmaxf(mm, p.part_ml[2 * (s * step + row)]);
-#pragma unroll
-    for (int x = LPR; x < 64; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
-    float ll = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = gr; s < p.splits; s += NG) {
-        const long at = s * step + row;
-        const float lp = p.part_ml[2 * at + 1];
-        if (lp == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - mm);
-        ll += lp * f;
-        acc += *reinterpret_cast<const f32x4*>(p.part_o + at * D + d) * f;
-    }
+    float total = 0.f;
+    if (live) {
+        float m[FOLD_MAX / 64], l[FOLD_MAX / 64], top = M_INIT;
 #pragma unroll
-    for (int x = LPR; x < 64; x *= 2) {
-        ll += __shfl_xor(ll, x, 64);
+        for (int j = 0; j < FOLD_MAX / 64; ++j) {
+            const int s = j * 64 + lane;
+            m[j] = M_INIT;
+            l[j] = 0.f;
+            if (s < p.splits) {
+                m[j] = p.part_ml[2 * (s * step + row)];
+                l[j] = p.part_ml[2 * (s * step + row) + 1];
+            }
+            top = fmaxf(top, m[j]);
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], x, 64);
+        for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+#pragma unroll
+        for (int j = 0; j < FOLD_MAX / 64; ++j) {
+            m[j] = l[j] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[j] - top);
+            total += l[j] * m[j];
+        }
+        total = wave_sum(total);
+#pragma unroll
+        for (int j = 0; j < FOLD_MAX / 64; ++j) {
+#pragma unroll 4
+            for (int s = (wave % W) * NG; s < 64; s += NG * W) {
+                if (j * 64 + s >= p.splits) break;
+                const float f = __shfl(m[j], s + gr, 64);      // 0 behind the last range
+                if (f != 0.f) acc += *reinterpret_cast<const f32x4*>(p.part_o + ((j * 64 + s + gr) * step + row) * D + d) * f;
+            }
+        }
+#pragma unroll
+        for (int x = LPR; x < 64; x *= 2)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], x, 64);
     }
-    if (gr == 0) {
-        const float inv = ll == 0.f ? 0.f : (1.0f / HALF) / ll;
+    if constexpr (W == 4) {
+        if (gr == 0) s_acc[wave][lane] = acc;
+        __syncthreads();
+        if (wave == 0 && gr == 0) acc = (s_acc[0][lane] + s_acc[1][lane]) + (s_acc[2][lane] + s_acc[3][lane]);
+    }
+    if (live && gr == 0 && wave % W == 0) {
+        const float inv = total == 0.f ? 0.f : (1.0f / HALF) / total;
         u32x2 w;
         w[0] = pack_h2<FMT, false>(acc[0] * inv, acc[1] * inv);
         w[1] = pack_h2<FMT, false>(acc[2] * inv, acc[3] * inv);
@@ -286,18 +304,12 @@ __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams 
     }
 }
 
-template <int D>
-int launch_fold(const SeqAttnParams& p, int fmt, bool paged, hipStream_t stream) {
-    const long rows = (long)p.B * p.max_q * p.Hq, n = (rows + 3) / 4;
-    if (n >= (1L << 31)) return -4;
-    const dim3 grid((unsigned)n), block(256);
-    if (fmt == FMT_F16) {
-        if (paged) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_F16, true>), grid, block, 0, stream, p);
-        else hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_F16, false>), grid, block, 0, stream, p);
-    } else {
-        if (paged) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_BF16, true>), grid, block, 0, stream, p);
-        else hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT_BF16, false>), grid, block, 0, stream, p);
-    }
+template <int D, int FMT, bool PAGED>
+int launch_fold(const SeqAttnParams& p, hipStream_t stream) {
+    const long rows = (long)p.B * p.max_q * p.Hq;
+    if (rows >= (1L << 31)) return -4;
+    if (rows <= 2048) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT, PAGED, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT, PAGED, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
 }
@@ -313,17 +325,20 @@ int launch_rows(const SeqAttnParams& p, int fmt, hipStream_t stream) {
     return 0;
 }
 
-// Up to 16 rows per (request, key head): the row kernel, its key ranges multiples of 256 keys, as many as give the chip 4
-// workgroups per CU.
+// Up to 16 rows per (request, key head): the row kernel.  Its key ranges are of one length, a multiple of 256 keys, whatever the
+// requests' own lengths, so that requests of different lengths fill the chip evenly; the range is as long as leaves about 2 500
+// work items (three to five rounds of the chip) if all requests had max_len tokens, and FOLD_MAX ranges at most.
 bool few_rows(long max_q, int G) { return max_q * G <= 16; }
 SeqPlan paged_plan(int B, long max_q, long max_len, int Hkv, int G, int D) {
     if (!few_rows(max_q, G)) return iggt_seq_tile_plan(B, max_q, max_len, Hkv, G, D);
-    const long pairs = (long)B * Hkv, most = (max_len + 255) / 256;
-    long s = (1024 + pairs - 1) / pairs;
-    if (s > most) s = most;
-    if (s > 64) s = 64;
-    if (s < 1) s = 1;
-    SeqPlan plan = {(int)s, false};
+    const long pairs = (long)B * Hkv, blocks = (max_len + 63) / 64;
+    long want = 2560 / pairs;
+    if (want > FOLD_MAX) want = FOLD_MAX;
+    if (want < 1) want = 1;
+    long range = ((blocks + want - 1) / want + 3) / 4 * 4;
+    if (range < 4) range = 4;
+    SeqPlan plan = {(int)((blocks + range - 1) / range), false, (int)range};
+    if (plan.splits < 1) plan.splits = 1;
     return plan;
 }
 
@@ -332,7 +347,12 @@ int page_shift_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 6
 }  // namespace
 
 int iggt_launch_seq_fold(const SeqAttnParams& p, int D, int fmt, bool paged, hipStream_t stream) {
-    return D == 64 ? launch_fold<64>(p, fmt, paged, stream) : launch_fold<128>(p, fmt, paged, stream);
+    if (fmt == FMT_F16) {
+        if (D == 64) return paged ? launch_fold<64, FMT_F16, true>(p, stream) : launch_fold<64, FMT_F16, false>(p, stream);
+        return paged ? launch_fold<128, FMT_F16, true>(p, stream) : launch_fold<128, FMT_F16, false>(p, stream);
+    }
+    if (D == 64) return paged ? launch_fold<64, FMT_BF16, true>(p, stream) : launch_fold<64, FMT_BF16, false>(p, stream);
+    return paged ? launch_fold<128, FMT_BF16, true>(p, stream) : launch_fold<128, FMT_BF16, false>(p, stream);
 }
 
 static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o, long o_rs, long o_hs, const void* k_codes,
@@ -359,6 +379,7 @@ static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o,
     p.scale_log2 = scale * 1.4426950408889634f;
     const SeqPlan plan = paged_plan(B, max_q, max_len, Hkv, p.G, D);
     p.splits = plan.splits;
+    p.range_blocks = plan.range_blocks;
     if (p.splits > 1) {
         const long n = (long)p.splits * B * max_q * Hq;
         if (ws == nullptr || ws_len < n * (D + 2) * 4 || (uintptr_t)ws % 16) return -5;

@@ -31,6 +31,7 @@ struct SeqAttnParams {
     int table_width, num_pages, page_shift;
     int B, Hq, Hkv, G, Tq, Tk, max_q, causal;
     int qtiles, splits;
+    int range_blocks;     // few rows: key range of a split in blocks of 64 keys
     float scale_log2;     // softmax scale * log2(e)
     // splits > 1: key range s of a row leaves its unnormalised sum [splits][B][max_q][Hq][D] and (maximum, row sum) here
     float* part_o;
@@ -38,6 +39,7 @@ struct SeqAttnParams {
 };
 
 constexpr float M_INIT = -3.0e38f;   // running maximum before the first key: finite, so that a masked score (-inf) gives 2^-inf = 0
+constexpr int FOLD_MAX = 128;        // key ranges a row is folded from at most
 constexpr float P_SHIFT_F16 = 8.0f;  // fp16 numerators are 2^(s - m + 8): the small ones stay normal; cancels in O / l
 
 struct SeqSpan {
@@ -128,5 +130,6 @@ int iggt_launch_seq_fold(const iggt_seq::SeqAttnParams& p, int D, int fmt, bool 
 struct SeqPlan {
     int splits;
     bool small;   // 128-row tiles where 256-row ones exist
+    int range_blocks;
 };
 SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D);

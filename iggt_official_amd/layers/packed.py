@@ -28,69 +28,71 @@ HEAD_DIMS = (64, 128)
 MAX_REQUESTS = 8192
 
 
-def _need(ok, what):
-    if not ok:
-        raise _C.HipExtensionError(what)
+# The checks run on every call of a few microseconds: conditions first, messages only where one fails.
+def _refuse(what):
+    raise _C.HipExtensionError(what)
 
 
 def _call(name, device, *args):
     """C entry on the current stream of `device`, whichever device is current."""
-    fn = getattr(_C.load(), name)
     index = device.index
-    if index == torch.cuda.current_device():
+    fn = getattr(_C.load(), name)
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    _C._check(rc, name)
+    if rc:
+        _C._check(rc, name)
 
 
 def _strides(name, t, step):
     """(row, head) strides of a [rows, heads, channels] operand; dimensions of one entry have none."""
-    rows, heads, dim = t.shape
     rs, hs, cs = t.stride()
-    rs, hs = (0 if rows <= 1 else rs), (0 if heads == 1 else hs)
-    _need(cs == 1 and rs % step == 0 and hs % step == 0 and t.data_ptr() % (2 * step) == 0,
-          f"{name}: channels have to be contiguous, strides multiples of {step} elements and the start aligned to {2 * step} bytes")
+    if t.shape[0] <= 1:
+        rs = 0
+    if t.shape[1] == 1:
+        hs = 0
+    if cs != 1 or rs % step or hs % step or t.data_ptr() % (2 * step):
+        _refuse(f"{name}: channels have to be contiguous, strides multiples of {step} elements and the start aligned to {2 * step} bytes")
     return rs, hs
 
 
-def _operands(q, out, **others):
-    """Checks that hold for both attentions; returns the output."""
-    _need(q.is_cuda, "IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
-    _need(q.dim() == 3 and q.dtype in _C.H16 and q.shape[2] in HEAD_DIMS, f"q: bf16 or fp16 [rows, heads, 64 | 128] expected, got {q.dtype} {tuple(q.shape)}")
-    grad = q.requires_grad
-    for name, t in others.items():
-        _need(t.device == q.device, f"{name} is on {t.device}, q on {q.device}")
-        grad = grad or t.requires_grad
-    _need(not (grad and torch.is_grad_enabled()), "packed / paged attention is forward only: an input requires gradients")
+def _query(q, out, grad):
+    """Checks of the query rows and of the output that hold for both attentions; returns the output."""
+    if not q.is_cuda:
+        _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
+    if q.dim() != 3 or q.dtype not in _C.H16 or q.shape[2] not in HEAD_DIMS:
+        _refuse(f"q: bf16 or fp16 [rows, heads, 64 | 128] expected, got {q.dtype} {tuple(q.shape)}")
+    if grad and torch.is_grad_enabled():
+        _refuse("packed / paged attention is forward only: an input requires gradients")
     if out is None:
         return torch.zeros_like(q, memory_format=torch.contiguous_format)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out has to have q's shape, type and device")
-    _need(all(n == 1 or s > 0 for n, s in zip(out.shape, out.stride())), "out is an expanded view")
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        _refuse("out has to have q's shape, type and device")
+    rs, hs, _ = out.stride()
+    if (rs == 0 and q.shape[0] > 1) or (hs == 0 and q.shape[1] > 1):
+        _refuse("out is an expanded view")
     return out
 
 
-def _index(name, t, shape, device):
-    _need(t.dtype == _INT and t.device == device and tuple(t.shape) == shape and t.is_contiguous(),
-          f"{name}: contiguous int32 {list(shape)} on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+def _index(name, t, n, device):
+    if t.dtype != _INT or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+        _refuse(f"{name}: contiguous int32 [{n}] on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _scale(scale, dim):
-    scale = dim ** -0.5 if scale is None else float(scale)
-    _need(0.0 < scale < float("inf"), f"softmax scale has to be positive and finite, got {scale}")
+    if scale is None:
+        return dim ** -0.5
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        _refuse(f"softmax scale has to be positive and finite, got {scale}")
     return scale
 
 
 @functools.lru_cache(maxsize=1024)
 def _ws_bytes(name, *sizes):
     return int(getattr(_C.load(), name)(*sizes))
-
-
-def _workspace(name, device, *sizes):
-    n = _ws_bytes(name, *sizes)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    return ws, (0 if ws is None else ws.data_ptr()), n
 
 
 def packed_attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, *, causal: bool = True, scale: Optional[float] = None,
@@ -101,25 +103,32 @@ def packed_attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, *, causal: boo
 
     max_q, max_k: the longest sequences' lengths or more (rows of a sequence past max_q are not computed).  out: rows that belong to
     no sequence are left as they are; without it they are 0."""
-    out = _operands(q, out, k=k, v=v)
+    out = _query(q, out, q.requires_grad or k.requires_grad or v.requires_grad)
+    device, dtype = q.device, q.dtype
     tq, hq, dim = q.shape
-    _need(k.dim() == 3 and k.shape == v.shape and k.dtype == q.dtype and v.dtype == q.dtype and k.shape[2] == dim,
-          f"k, v: {q.dtype} [keys, heads, {dim}] expected, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != dtype or v.dtype != dtype or k.shape[2] != dim or k.device != device or v.device != device:
+        _refuse(f"k, v: {dtype} [keys, heads, {dim}] on {device} expected, got {k.dtype} {tuple(k.shape)} on {k.device} and {v.dtype} {tuple(v.shape)} on {v.device}")
     tk, hkv, _ = k.shape
-    _need(hkv > 0 and hq > 0 and hq % hkv == 0, f"{hq} query heads are no multiple of {hkv} key heads")
-    batch = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
-    _need(batch >= 0, "cu_q: one entry more than there are sequences expected")
-    _index("cu_q", cu_q, (batch + 1,), q.device), _index("cu_k", cu_k, (batch + 1,), q.device)
+    if hkv == 0 or hq == 0 or hq % hkv:
+        _refuse(f"{hq} query heads are no multiple of {hkv} key heads")
+    batch = cu_q.numel() - 1
+    if batch < 0:
+        _refuse("cu_q: one entry more than there are sequences expected")
+    _index("cu_q", cu_q, batch + 1, device)
+    _index("cu_k", cu_k, batch + 1, device)
     max_q, max_k = min(int(max_q), tq), min(int(max_k), tk)
-    _need(max_q >= 0 and max_k >= 0, "max_q and max_k are lengths")
+    if max_q < 0 or max_k < 0:
+        _refuse("max_q and max_k are lengths")
     scale = _scale(scale, dim)
+    strides = _strides("q", q, 8), _strides("k", k, 8), _strides("v", v, 8), _strides("out", out, 4)
     if batch == 0 or max_q == 0:
         return out
-    ws, ws_ptr, n = _workspace("iggt_packed_attn_ws_bytes", q.device, batch, max_q, max_k, hq, hkv, dim)
-    _call("iggt_packed_attn_" + ("f16" if q.dtype == torch.float16 else "bf16"), q.device,
-          q.data_ptr(), *_strides("q", q, 8), k.data_ptr(), *_strides("k", k, 8), v.data_ptr(), *_strides("v", v, 8),
-          out.data_ptr(), *_strides("out", out, 4), cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, max_q, max_k, hq, hkv, dim,
-          scale, int(causal), ws_ptr, n)
+    n = _ws_bytes("iggt_packed_attn_ws_bytes", batch, max_q, max_k, hq, hkv, dim)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    _call("iggt_packed_attn_f16" if dtype == torch.float16 else "iggt_packed_attn_bf16", device,
+          q.data_ptr(), *strides[0], k.data_ptr(), *strides[1], v.data_ptr(), *strides[2], out.data_ptr(), *strides[3],
+          cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, max_q, max_k, hq, hkv, dim, scale, int(causal),
+          0 if ws is None else ws.data_ptr(), n)
     return out
 
 
@@ -133,8 +142,8 @@ class Pages(NamedTuple):
 
     @staticmethod
     def empty(pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda") -> "Pages":
-        _need(page in PAGE_SIZES and head_dim in HEAD_DIMS and pages >= 0 and kv_heads > 0,
-              f"pages of {PAGE_SIZES} tokens and head dims {HEAD_DIMS} expected, got {page} and {head_dim}")
+        if page not in PAGE_SIZES or head_dim not in HEAD_DIMS or pages < 0 or kv_heads <= 0:
+            _refuse(f"pages of {PAGE_SIZES} tokens and head dims {HEAD_DIMS} expected, got {page} and {head_dim}")
         make = functools.partial(torch.zeros, dtype=torch.uint8, device=device)
         return Pages(make(pages, kv_heads, page, head_dim), make(pages, kv_heads), make(pages, kv_heads, page // 16, head_dim, 16),
                      make(pages, kv_heads))
@@ -142,14 +151,15 @@ class Pages(NamedTuple):
 
 def _pages(pages, device):
     """(number of pages, key heads, page size, head dim) of a checked cache."""
-    k = pages.k_codes
-    _need(k.dim() == 4 and k.shape[2] in PAGE_SIZES and k.shape[3] in HEAD_DIMS,
-          f"K codes: [pages, heads, {PAGE_SIZES}, {HEAD_DIMS}] expected, got {tuple(k.shape)}")
-    n, heads, page, dim = k.shape
-    for t, shape in ((k, k.shape), (pages.k_scale, (n, heads)), (pages.v_codes, (n, heads, page // 16, dim, 16)), (pages.v_scale, (n, heads))):
-        _need(t.dtype == torch.uint8 and t.shape == shape and t.is_contiguous() and t.device == device,
-              f"cache buffers: contiguous uint8 {tuple(shape)} on {device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    _need(n * page < 2 ** 31, "more than 2^31 slots")
+    k, ks, v, vs = pages
+    n, heads, page, dim = k.shape if k.dim() == 4 else (0, 0, 0, 0)
+    if page not in PAGE_SIZES or dim not in HEAD_DIMS or heads == 0 or n * page >= 2 ** 31:
+        _refuse(f"K codes: [pages, heads, {PAGE_SIZES}, {HEAD_DIMS}] expected, got {tuple(k.shape)}")
+    if ks.shape != (n, heads) or vs.shape != (n, heads) or v.shape != (n, heads, page // 16, dim, 16):
+        _refuse(f"cache buffers do not belong together: {[tuple(t.shape) for t in pages]}")
+    for t in pages:
+        if t.dtype != torch.uint8 or t.device != device or not t.is_contiguous():
+            _refuse(f"cache buffers: contiguous uint8 on {device} expected, got {t.dtype} on {t.device}")
     return n, heads, page, dim
 
 
@@ -158,14 +168,18 @@ def append_pages(pages: Pages, k, v, slots):
     not in the cache are skipped).  Rows of one page have to be one run of consecutive slots, as plan_pages gives them: a page that
     appears in two runs of one call has no defined content.  The scale of a page is the least power of two that holds its largest
     finite value, and never falls while the page is being filled; held codes are rewritten when it grows."""
-    _need(k.is_cuda and k.dim() == 3 and k.dtype in _C.H16, "k: bf16 or fp16 [tokens, key heads, D] on a ROCm device expected (no CPU fallback)")
-    n, heads, page, dim = _pages(pages, k.device)
-    _need(v.shape == k.shape and v.dtype == k.dtype and v.device == k.device and tuple(k.shape[1:]) == (heads, dim),
-          f"k, v: [tokens, {heads}, {dim}] of one type expected, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    _need(not ((k.requires_grad or v.requires_grad) and torch.is_grad_enabled()), "append_pages is forward only: an input requires gradients")
-    _index("slots", slots, (k.shape[0],), k.device)
-    _call("iggt_append_pages_" + ("f16" if k.dtype == torch.float16 else "bf16"), k.device,
-          k.data_ptr(), *_strides("k", k, 8), v.data_ptr(), *_strides("v", v, 8), slots.data_ptr(), k.shape[0],
+    device, dtype = k.device, k.dtype
+    if not k.is_cuda or k.dim() != 3 or dtype not in _C.H16:
+        _refuse("k: bf16 or fp16 [tokens, key heads, D] on a ROCm device expected (no CPU fallback)")
+    n, heads, page, dim = _pages(pages, device)
+    tokens = k.shape[0]
+    if k.shape != (tokens, heads, dim) or v.shape != k.shape or v.dtype != dtype or v.device != device:
+        _refuse(f"k, v: [tokens, {heads}, {dim}] of one type expected, got {tuple(k.shape)} {dtype} and {tuple(v.shape)} {v.dtype}")
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _refuse("append_pages is forward only: an input requires gradients")
+    _index("slots", slots, tokens, device)
+    _call("iggt_append_pages_f16" if dtype == torch.float16 else "iggt_append_pages_bf16", device,
+          k.data_ptr(), *_strides("k", k, 8), v.data_ptr(), *_strides("v", v, 8), slots.data_ptr(), tokens,
           pages.k_codes.data_ptr(), pages.k_scale.data_ptr(), pages.v_codes.data_ptr(), pages.v_scale.data_ptr(), n, page, heads, dim)
     return pages
 
@@ -178,31 +192,46 @@ def paged_attention(q, pages: Pages, tables, lens, max_q: int, max_len: int, *, 
 
     max_q, max_len: the largest number of rows, of tokens, or more.  Tokens on a page that does not exist count as not there.  out:
     as in packed_attention."""
-    out = _operands(q, out, tables=tables, lens=lens)
+    out = _query(q, out, q.requires_grad)
+    device, dtype = q.device, q.dtype
     tq, hq, dim = q.shape
-    n, hkv, page, d = _pages(pages, q.device)
-    _need(d == dim and hq > 0 and hq % hkv == 0, f"q has {hq} heads of {dim}, the cache {hkv} of {d}")
-    _need(tables.dim() == 2 and tables.dtype == _INT and (tables.shape[1] <= 1 or tables.stride(1) == 1),
-          "tables: int32 [requests, pages of the longest] with contiguous rows expected")
-    batch, width = tables.shape
-    _index("lens", lens, (batch,), q.device)
-    max_q = min(int(max_q), tq)
-    if cu_q is None:
-        _need(max_q <= 1 and tq >= batch, "without cu_q there is one row per request")
-    else:
-        _index("cu_q", cu_q, (batch + 1,), q.device)
-    max_len = min(int(max_len), width * page)
-    _need(max_q >= 0 and max_len >= 0 and width * page < 2 ** 31, "max_q and max_len are lengths")
+    n, hkv, page, d = _pages(pages, device)
+    if d != dim or hq == 0 or hq % hkv:
+        _refuse(f"q has {hq} heads of {dim}, the cache {hkv} of {d}")
+    batch, width, stride = _tables(tables, device, page)
+    _index("lens", lens, batch, device)
+    max_q, max_len = min(int(max_q), tq), min(int(max_len), width * page)
+    if max_q < 0 or max_len < 0:
+        _refuse("max_q and max_len are lengths")
+    if cu_q is not None:
+        _index("cu_q", cu_q, batch + 1, device)
+    elif max_q > 1 or tq < batch:
+        _refuse("without cu_q there is one row per request")
     scale = _scale(scale, dim)
+    strides = _strides("q", q, 8), _strides("out", out, 4)
     if batch == 0 or max_q == 0:
         return out
-    ws, ws_ptr, nbytes = _workspace("iggt_paged_attn_ws_bytes", q.device, batch, max_q, max_len, hq, hkv, dim)
-    _call("iggt_paged_attn_" + ("f16" if q.dtype == torch.float16 else "bf16"), q.device,
-          q.data_ptr(), *_strides("q", q, 8), out.data_ptr(), *_strides("out", out, 4),
+    nbytes = _ws_bytes("iggt_paged_attn_ws_bytes", batch, max_q, max_len, hq, hkv, dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _call("iggt_paged_attn_f16" if dtype == torch.float16 else "iggt_paged_attn_bf16", device,
+          q.data_ptr(), *strides[0], out.data_ptr(), *strides[1],
           pages.k_codes.data_ptr(), pages.k_scale.data_ptr(), pages.v_codes.data_ptr(), pages.v_scale.data_ptr(), n, page,
-          tables.data_ptr(), tables.stride(0), width, lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), batch, tq, max_q,
-          max_len, hq, hkv, dim, scale, int(causal), ws_ptr, nbytes)
+          tables.data_ptr(), stride, width, lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), batch, tq, max_q,
+          max_len, hq, hkv, dim, scale, int(causal), 0 if ws is None else ws.data_ptr(), nbytes)
     return out
+
+
+def _tables(tables, device, page):
+    """(requests, width, row stride) of checked block tables."""
+    if tables.dim() != 2 or tables.dtype != _INT or tables.device != device:
+        _refuse(f"tables: int32 [requests, pages of the longest] on {device} expected, got {tables.dtype} {tuple(tables.shape)} on {tables.device}")
+    requests, width = tables.shape
+    rs, cs = tables.stride()
+    if (width > 1 and cs != 1) or (requests > 1 and rs < width):
+        _refuse("tables: contiguous rows that do not overlap expected")
+    if width * page >= 2 ** 31 - 128:
+        _refuse("more than 2^31 slots")
+    return requests, width, rs
 
 
 def plan_pages(tables, ring, counters, lens, new_lens, page: int, tokens: int):
@@ -215,27 +244,26 @@ def plan_pages(tables, ring, counters, lens, new_lens, page: int, tokens: int):
     added tokens in request order, -1 behind the last, request b's at starts[b] .. starts[b + 1].  `missing` pages > 0 (or -1: `tokens` is
     too small) means that no request has grown in this step."""
     device = tables.device
-    _need(tables.is_cuda, "IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
-    _need(page in PAGE_SIZES, f"pages hold {PAGE_SIZES} tokens, not {page}")
-    _need(tables.dim() == 2 and tables.dtype == _INT and (tables.shape[1] <= 1 or tables.stride(1) == 1) and (tables.shape[0] <= 1 or tables.stride(0) >= tables.shape[1]),
-          "tables: int32 [requests, pages of the longest] with contiguous rows expected")
-    requests, width = tables.shape
-    tokens = int(tokens)
-    _need(requests <= MAX_REQUESTS and tokens >= 0, f"at most {MAX_REQUESTS} requests")
-    _need(width * page < 2 ** 31 - 128 and ring.numel() * page < 2 ** 31, "more than 2^31 slots")
-    _index("ring", ring, (ring.numel(),), device)
-    _need(counters.dtype == _INT and counters.device == device and counters.dim() == 1 and counters.numel() >= 2 and counters.is_contiguous(),
-          "counters: int32 (head, count, ...) expected")
-    _index("lens", lens, (requests,), device), _index("new_lens", new_lens, (requests,), device)
-    # one allocation for the four outputs, each 16-byte aligned
-    at = [0]
-    for n in (requests + 1, requests, 3, tokens):
-        at.append(at[-1] + (n + 3) // 4 * 4)
-    buf = torch.empty(at[-1], dtype=_INT, device=device)
-    starts, next_lens, next_counters, slots = (buf[a:a + n] for a, n in zip(at, (requests + 1, requests, 3, tokens)))
+    if not tables.is_cuda:
+        _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
+    if page not in PAGE_SIZES:
+        _refuse(f"pages hold {PAGE_SIZES} tokens, not {page}")
+    requests, width, stride = _tables(tables, device, page)
+    tokens, size = int(tokens), ring.numel()
+    if requests > MAX_REQUESTS or tokens < 0 or size * page >= 2 ** 31:
+        _refuse(f"at most {MAX_REQUESTS} requests and 2^31 slots")
+    _index("ring", ring, size, device)
+    if counters.numel() < 2:
+        _refuse("counters: int32 (head, count, ...) expected")
+    _index("counters", counters, counters.numel(), device)
+    _index("lens", lens, requests, device)
+    _index("new_lens", new_lens, requests, device)
+    buf = torch.empty(2 * requests + 4 + tokens, dtype=_INT, device=device)     # one allocation for the four outputs
+    starts, next_lens, next_counters, slots = buf.split((requests + 1, requests, 3, tokens))
     base = buf.data_ptr()
-    _call("iggt_plan_pages", device, tables.data_ptr(), tables.stride(0), requests, width, ring.data_ptr(), ring.numel(),
-          counters.data_ptr(), lens.data_ptr(), new_lens.data_ptr(), page, base, base + 4 * at[1], base + 4 * at[2], base + 4 * at[3], tokens)
+    _call("iggt_plan_pages", device, tables.data_ptr(), stride, requests, width, ring.data_ptr(), size,
+          counters.data_ptr(), lens.data_ptr(), new_lens.data_ptr(), page, base, base + 4 * (requests + 1), base + 4 * (2 * requests + 1),
+          base + 4 * (2 * requests + 4), tokens)
     return tables, ring, starts, next_lens, next_counters, slots
 
 
@@ -251,8 +279,8 @@ class PagedKVCache:
     a step goes on where the last replay ended."""
 
     def __init__(self, requests: int, longest: int, pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda"):
-        _need(page in PAGE_SIZES, f"pages hold {PAGE_SIZES} tokens, not {page}")
-        _need(0 < requests <= MAX_REQUESTS and longest > 0 and pages > 0, "requests, longest and pages have to be positive")
+        if not 0 < requests <= MAX_REQUESTS or longest <= 0 or pages <= 0:
+            _refuse(f"up to {MAX_REQUESTS} requests, of one token or more, and one page or more expected")
         self.page = page
         self.pages = Pages.empty(pages, kv_heads, head_dim, page, device)
         device = self.pages.k_codes.device
