@@ -160,15 +160,16 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     uint32_t have_next = 0xf, have = 0xf;       // which 16-key groups of the tile have a page
     // a wave's piece i lies in one 16-key group: one table entry, loaded a tile ahead (lane l: group l & 3), serves its K and its V
     const int psub = D == 64 ? wave : wave >> 1;
-    int pid = -1;
-    auto look_up = [&](int t) { pid = page_of(p, b, t * 64 + (lane & 3) * 16); };
+    int pid = 0;
+    auto look_up = [&](int t) { pid = page_entry(p, b, t * 64 + (lane & 3) * 16); };
     auto fetch = [&](int t) {
-        have_next = (uint32_t)__ballot(pid >= 0) & 0xfu;
+        have_next = (uint32_t)__ballot(page_ok(p, pid)) & 0xfu;
         const int pmask = (1 << p.page_shift) - 1;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
             const int sub = psub + 2 * i;
-            const long head = (long)max(__builtin_amdgcn_readlane(pid, sub), 0) * p.Hkv + h;
+            const int id = __builtin_amdgcn_readlane(pid, sub);
+            const long head = (long)(page_ok(p, id) ? id : 0) * p.Hkv + h;
             const long at = ((head << p.page_shift) + ((t * 64 + sub * 16) & pmask)) * D;      // of the group's K rows, and of its V
             const int in = D == 64 ? lane * 16 : ((wave & 1) * 64 + lane) * 16;
             k8r[i] = *reinterpret_cast<const u32x4*>(p.k8 + at + in);
@@ -362,20 +363,19 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         if constexpr (PAGED) {
             look_up(t0);
             fetch(t0);
-            if (t0 + 1 < t1) look_up(t0 + 1);
+            look_up(t0 + 1);
             stage(t0 & 1);
         } else {
             dma(t0, t0 & 1);
         }
         __syncthreads();   // (drains the DMA as well)
         for (int mt = t0; mt < t1; ++mt) {
-            if (mt + 1 < t1) {
-                if constexpr (PAGED) {
-                    fetch(mt + 1);
-                    if (mt + 2 < t1) look_up(mt + 2);
-                } else {
-                    dma(mt + 1, (mt + 1) & 1);
-                }
+            if constexpr (PAGED) {
+                // (the last tile fetches itself again: a branch here would make every wait one for all loads)
+                fetch(min(mt + 1, t1 - 1));
+                look_up(mt + 2);
+            } else {
+                if (mt + 1 < t1) dma(mt + 1, (mt + 1) & 1);
             }
 #pragma unroll
             for (int sub = 0; sub < KVM; ++sub) {
@@ -501,6 +501,7 @@ static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const v
                            int Tk, int max_q, int max_k, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
                            void* stream) {
     if (B < 0 || Tq < 0 || Tk < 0 || max_q < 0 || max_k < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
+    if (Tk >= 0x7fffffff - 1024) return -1;
     if ((q_rs | q_hs | k_rs | k_hs | v_rs | v_hs) % 8 || (o_rs | o_hs) % 4) return -2;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || (uintptr_t)o % 8) return -2;
     if (k_rs < 0 || v_rs < 0 || k_rs >= (1L << 24) || v_rs >= (1L << 24)) return -2;   // 64 rows in 32-bit byte offsets

@@ -26,8 +26,9 @@ IGGT_DEVINL f32x4 mfma16h(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-template <int D, int FMT>
-__global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnParams p) {
+// DRAFT: several tokens per request, so that near the end a key may be seen by some rows only.
+template <int D, int FMT, bool DRAFT>
+__global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const SeqAttnParams p) {
     constexpr int NC = D / 64, NDT = D / 16;
     constexpr float HALF = FMT == FMT_F16 ? 0.5f : 1.0f;   // fp16 holds half of V's values (a code at the top of its range is 2^16)
     __shared__ float s_o[4][16][D + 4];
@@ -65,37 +66,39 @@ __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnPara
     const int pmask = (1 << p.page_shift) - 1;
     const int a_sub = n >> 2, a_key = n & 3;
     u32x4 kc[4][NC], vc[NDT];
-    int k_page, v_page;        // page of the lane's K rows / of its V keys in the block being loaded
-    auto pages = [&](int blk, int& kp, int& vp) {
-        kp = page_of(p, b, blk * 64 + a_sub * 16);
-        vp = page_of(p, b, blk * 64 + g * 16);
+    // Loads complete in the order they are issued, so nothing may wait for one that is younger than what is meant to stay in flight:
+    // page ids are loaded two blocks ahead, the scales in front of the K codes of their block.
+    int kp = 0, vp = 0, kp1 = 0, vp1 = 0;          // table entries of the lane's K rows / of its V keys: this block, the next one
+    uint32_t kb = 127, vb = 127;                   // their scale bytes, of the group g whose scores the lane holds
+    auto pages = [&](int blk, int& k_page, int& v_page) {
+        k_page = page_entry(p, b, blk * 64 + a_sub * 16);
+        v_page = page_entry(p, b, blk * 64 + g * 16);
     };
-    auto load_k = [&](int blk, int page) {
-        const uint8_t* src = p.k8 + (((((long)max(page, 0) * p.Hkv + h) << p.page_shift) + ((blk * 64 + a_sub * 16) & pmask) + a_key) * D) + 16 * g;
+    auto load_k = [&](int blk, int k_page, int v_page) {
+        const long sidx = (long)(page_ok(p, v_page) ? v_page : 0) * p.Hkv + h;
+        kb = p.k_scale[sidx];
+        vb = p.v_scale[sidx];
+        const uint8_t* src = p.k8 + (((((long)(page_ok(p, k_page) ? k_page : 0) * p.Hkv + h) << p.page_shift) + ((blk * 64 + a_sub * 16) & pmask) + a_key) * D) + 16 * g;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < NC; ++c) kc[t][c] = *reinterpret_cast<const u32x4*>(src + (4 * t) * D + 64 * c);
     };
     auto load_v = [&](int blk, int page) {
-        const uint8_t* src = p.v8 + (((((long)max(page, 0) * p.Hkv + h) << p.page_shift) + ((blk * 64 + g * 16) & pmask)) * D) + n * 16;
+        const uint8_t* src = p.v8 + (((((long)(page_ok(p, page) ? page : 0) * p.Hkv + h) << p.page_shift) + ((blk * 64 + g * 16) & pmask)) * D) + n * 16;
 #pragma unroll
         for (int i = 0; i < NDT; ++i) vc[i] = *reinterpret_cast<const u32x4*>(src + 256 * i);
     };
 
     int blk = b0 + wave;
     if (blk < b1) {
-        pages(blk, k_page, v_page);
-        load_k(blk, k_page);
+        pages(blk, kp, vp);
+        pages(blk + 4, kp1, vp1);
+        load_k(blk, kp, vp);
     }
     for (; blk < b1; blk += 4) {
-        const int vp = v_page;
         load_v(blk, vp);
-        const long sidx = (long)max(vp, 0) * p.Hkv + h;
-        const float ks = scale_of(p.k_scale[sidx]) * p.scale_log2, vs = scale_of(p.v_scale[sidx]) * HALF;
-        const bool more = blk + 4 < b1;
-        if (more) pages(blk + 4, k_page, v_page);
-
+        const float ks = scale_of(kb) * p.scale_log2, vs = scale_of(vb) * HALF;
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -108,7 +111,17 @@ __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnPara
                 s[t] = mfma16h<FMT>(hi, qf[c][1], s[t]);
             }
         }
-        if (more) load_k(blk + 4, k_page);
+        const int here = vp, kp0 = kp;
+        kp = kp1;
+        vp = vp1;
+        // (the last block loads itself again: with a branch here every later wait would be one for all loads)
+        const int next = blk + 4 < b1 ? blk + 4 : blk;
+        if (blk + 4 >= b1) {
+            kp = kp0;
+            vp = here;
+        }
+        pages(blk + 8, kp1, vp1);
+        load_k(next, kp, vp);
 
         float e[16];
 #pragma unroll
@@ -116,8 +129,8 @@ __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnPara
 #pragma unroll
             for (int r = 0; r < 4; ++r) e[4 * t + r] = s[t][r] * ks;
         const int key0 = blk * 64 + g * 16;
-        const bool edge = blk * 64 + 64 > first || __any(vp < 0);
-        const int seen = vp < 0 ? 0 : lim - key0;       // of the lane's 16 keys, the first `seen` count for its row
+        const bool edge = blk * 64 + 64 > first || __any(!page_ok(p, here));
+        const int seen = !page_ok(p, here) ? 0 : lim - key0;       // of the lane's 16 keys, the first `seen` count for its row
         if (edge) {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -143,18 +156,26 @@ __global__ __launch_bounds__(256, 2) void seq_attn_rows_kernel(const SeqAttnPara
             l += e[j];
         }
         const bf16x8 p0 = pack8f<FMT>(e), p1 = pack8f<FMT>(e + 8);
+        // codes 0x7f / 0xff are NaN (e4m3 has no infinity) and 0 * NaN is one: what lies behind the last key (whatever the page held) is
+        // zeroed, what only some rows see is found here
         bool bad = false;
         if (edge) {
-            // codes 0x7f / 0xff are NaN (e4m3 has no infinity): behind the end they are whatever the page held, before it they belong
-            // to rows that see them
-            uint32_t nan = 0;
+            const int held = !page_ok(p, here) ? 0 : kend - key0;
 #pragma unroll
-            for (int i = 0; i < NDT; ++i)
+            for (int w = 0; w < 4; ++w) {
+                const int keep = min(max(held - 4 * w, 0), 4);
+                const uint32_t bytes = keep == 4 ? ~0u : (1u << (8 * keep)) - 1u;
+                uint32_t nan = 0;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) nan |= ((vc[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-            bad = __any(nan != 0);
+                for (int i = 0; i < NDT; ++i) {
+                    vc[i][w] &= bytes;
+                    if (DRAFT) nan |= ((vc[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                }
+                if (DRAFT) bad = bad || nan != 0;
+            }
+            if (DRAFT) bad = __any(bad);
         }
-        if (!bad) {
+        if (!DRAFT || !bad) {
 #pragma unroll
             for (int i = 0; i < NDT; ++i) {
                 bf16x8 lo, hi;
@@ -278,7 +299,6 @@ __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams 
         total = wave_sum(total);
 #pragma unroll
         for (int j = 0; j < FOLD_MAX / 64; ++j) {
-#pragma unroll 4
             for (int s = (wave % W) * NG; s < 64; s += NG * W) {
                 if (j * 64 + s >= p.splits) break;
                 const float f = __shfl(m[j], s + gr, 64);      // 0 behind the last range
@@ -319,8 +339,13 @@ int launch_rows(const SeqAttnParams& p, int fmt, hipStream_t stream) {
     const long n = (long)p.splits * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
     const dim3 grid((unsigned)n), block(256);
-    if (fmt == FMT_F16) hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_F16>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_BF16>), grid, block, 0, stream, p);
+    if (fmt == FMT_F16) {
+        if (p.max_q == 1) hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_F16, false>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_F16, true>), grid, block, 0, stream, p);
+    } else {
+        if (p.max_q == 1) hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_BF16, false>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_BF16, true>), grid, block, 0, stream, p);
+    }
     IGGT_CHECK_LAUNCH();
     return 0;
 }
@@ -363,7 +388,7 @@ static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o,
     const int shift = page_shift_of(page);
     if (B < 0 || Tq < 0 || max_q < 0 || max_len < 0 || num_pages < 0 || table_width < 0 || shift < 0) return -1;
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
-    if ((long)table_width * page >= (1L << 31) || (cu_q == nullptr && max_q > 1)) return -1;
+    if ((long)table_width * page >= (1L << 31) - 1024 || (cu_q == nullptr && max_q > 1)) return -1;
     if ((q_rs | q_hs) % 8 || (o_rs | o_hs) % 4 || (uintptr_t)q % 16 || (uintptr_t)o % 8) return -2;
     if (((uintptr_t)k_codes | (uintptr_t)v_codes) % 16) return -2;
     if (!(scale > 0.f)) return -3;

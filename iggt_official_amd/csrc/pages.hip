@@ -356,7 +356,7 @@ int iggt_plan_pages(int* tables, long table_stride, int requests, int table_widt
                     int num_slots, void* stream) {
     const int shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
     if (requests < 0 || requests > PLAN_MAX_REQUESTS || table_width < 0 || num_pages < 0 || num_slots < 0 || shift < 0) return -1;
-    if (((long)table_width << shift) >= (1L << 31) - 128 || ((long)num_pages << shift) >= (1L << 31)) return -1;
+    if (((long)table_width << shift) >= (1L << 31) - 1024 || ((long)num_pages << shift) >= (1L << 31)) return -1;
     PlanParams p = {tables, table_stride, requests, table_width, ring, num_pages, counters, lens, new_lens, shift, starts,
                     next_lens, next_counters, slots, num_slots};
     // every workgroup repeats the prefix sums (microseconds), so only as many as the slots keep busy

@@ -68,12 +68,12 @@ IGGT_DEVINL SeqSpan seq_span(const SeqAttnParams& p, int b) {
     return s;
 }
 
-// page of token block `at` of request b; -1: no such page (keys of it count as not there)
-IGGT_DEVINL int page_of(const SeqAttnParams& p, int b, int at) {
-    if ((at >> p.page_shift) >= p.table_width) return -1;
-    const int id = p.tables[(long)b * p.table_stride + (at >> p.page_shift)];
-    return (unsigned)id < (unsigned)p.num_pages ? id : -1;
+// Table entry of the page of token `at` of request b (lk > 0, so the table has an entry; tokens behind its end read the last one and
+// are masked by their position).  The entry is not looked at here: a check would wait for the load.
+IGGT_DEVINL int page_entry(const SeqAttnParams& p, int b, int at) {
+    return p.tables[(long)b * p.table_stride + min((int)((unsigned)at >> p.page_shift), p.table_width - 1)];
 }
+IGGT_DEVINL bool page_ok(const SeqAttnParams& p, int id) { return (unsigned)id < (unsigned)p.num_pages; }
 
 // 16 e4m3 codes -> two fragments of 8 in the 16-bit operand type, times 2^(e - 127) (a power of two, so bf16 is exact; fp16 is
 // exact down to its subnormal step).  The instruction takes the scale as a float of which it reads the exponent.

@@ -229,7 +229,7 @@ def _tables(tables, device, page):
     rs, cs = tables.stride()
     if (width > 1 and cs != 1) or (requests > 1 and rs < width):
         _refuse("tables: contiguous rows that do not overlap expected")
-    if width * page >= 2 ** 31 - 128:
+    if width * page >= 2 ** 31 - 1024:
         _refuse("more than 2^31 slots")
     return requests, width, rs
 
