@@ -23,10 +23,25 @@ namespace {
 
 constexpr float DEFER_THR = 4.0f;
 
+// 16 bytes per lane from base + off straight into LDS at lds + 16 * lane (both uniform).  Inline assembly because the compiler's own
+// bookkeeping waits for every such load in flight before the next LDS read of the kernel, which is the next tile's arrival before this
+// tile's work.  No register is written, so nothing but the caller's arrive() has to know when it is done.
+IGGT_DEVINL void lds_load16(const void* base, uint32_t off, const char* lds) {
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(off), "s"(base), "s"(at) : "memory");   // (m0 is reserved: the compiler holds no value in it here)
+}
+// all of this wave's LDS loads have arrived, and every wave of the workgroup has come here
+IGGT_DEVINL void arrive() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // Order of the work items.  Longest first, so that the last ones to start are short: under a causal mask the last query tiles, else
 // the sequences by their number of keys (up to 64 of them: ranked here, one lane each).  Key heads innermost: consecutive workgroups
 // go to the XCDs in turn, so one head's tiles share an L2.  Where (sequence, head) pairs are a multiple of 8 but heads are not, an
-// XCD would keep one sequence for good: the pairs move on by one every 16th of the tiles.
+// XCD would keep one sequence for good: the pairs move on by one every 8 tiles (grouped prompts of 12 001 and 7 645 tokens, 8 pairs:
+// 932 us in place, 879 moved with every tile, 850 with every fourth, 845 every eighth: moving balances, staying shares the L2).
 template <bool PAGED>
 IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt, int& b, int& h) {
     int w = blockIdx.x;
@@ -37,7 +52,7 @@ IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt
         split = w % p.splits;
         const int at = w / p.splits;
         qt = p.qtiles - 1 - at;
-        pair = (pair + at / ((p.qtiles >> 4) + 1)) % npairs;
+        pair = (pair + at / min(max(p.qtiles >> 4, 1), 8)) % npairs;
         b = pair / p.Hkv;
         h = pair - b * p.Hkv;
     } else {
@@ -100,53 +115,45 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         for (int kc = 0; kc < NKC; ++kc) qf[qb][kc] = *reinterpret_cast<const bf16x8*>(src + 16 * kc);
     }
 
+    // the query fragments arrive here, so that no use of them in the tile loop waits for loads in flight
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int kc = 0; kc < NKC; ++kc) {
+            u32x4 w = __builtin_bit_cast(u32x4, qf[qb][kc]);
+            asm volatile("" : "+v"(w));
+            qf[qb][kc] = __builtin_bit_cast(bf16x8, w);
+        }
+
     // ---- staging.  16-bit: LDS-DMA, 1 KiB per wave and instruction; the row-image swizzles are applied to the source piece, rows
     //      past the end are clamped to the last key (masked; see the file comment for values that are not finite).
-    typedef __attribute__((address_space(1))) const void gptr_t;
-    typedef __attribute__((address_space(3))) void lptr_t;
     constexpr int RPC = 1024 / ROWB;            // rows of a 1 KiB chunk
     constexpr int CPW = K_BYTES / 1024 / 4;     // chunks per wave
     const bf16_t* kb_ptr = nullptr;
     const bf16_t* vb_ptr = nullptr;
-    int drow[CPW], kcol[CPW], vcol[CPW];        // row and swizzled byte column of the lane's piece in each of its chunks
-    uint32_t koffs[CPW], voffs[CPW];            // their byte offsets within a tile (host: a tile spans less than 2^32)
+    // the lane's piece of chunk i is in row wave CPW RPC + i RPC + lane / SLOTS of the tile, at the swizzled byte column kcol ^ flip(i) of
+    // K and vcol of V
+    const int drow = wave * (CPW * RPC) + lane / SLOTS, pos = lane % SLOTS;
+    const int kcol = (D == 64 ? pos ^ ((drow >> 1) & 7) : pos ^ (drow & 15)) * 16;
+    const int vcol = (D == 64 ? (((pos >> 1) ^ (drow & 2)) << 1) | (pos & 1) : (((pos >> 1) ^ ((drow & 3) << 1)) << 1) | (pos & 1)) * 16;
+    static_assert(RPC * CPW == 16, "a wave's rows begin at a multiple of 16");
+    uint32_t koff0 = 0, voff0 = 0;              // byte offset of the first chunk's piece (host: a tile spans less than 2^32)
     if constexpr (!PAGED) {
         kb_ptr = p.k + (long)sp.k0 * p.k_rs + (long)h * p.k_hs;
         vb_ptr = p.v + (long)sp.k0 * p.v_rs + (long)h * p.v_hs;
+        koff0 = (uint32_t)drow * (uint32_t)(2 * p.k_rs);
+        voff0 = (uint32_t)drow * (uint32_t)(2 * p.v_rs) + vcol;
+    }
+    auto dma = [&](bool V, int t, char* dst) {       // one 64-key tile of K or of V
+        const long rs = V ? p.v_rs : p.k_rs;
+        const char* src = reinterpret_cast<const char*>((V ? vb_ptr : kb_ptr) + (long)t * 64 * rs);
+        const int left = sp.lk - 1 - t * 64;
 #pragma unroll
         for (int i = 0; i < CPW; ++i) {
-            const int r = (wave * CPW + i) * RPC + lane / SLOTS, pos = lane % SLOTS;
-            drow[i] = r;
-            kcol[i] = (D == 64 ? pos ^ ((r >> 1) & 7) : pos ^ (r & 15)) * 16;
-            vcol[i] = (D == 64 ? (((pos >> 1) ^ (r & 2)) << 1) | (pos & 1) : (((pos >> 1) ^ ((r & 3) << 1)) << 1) | (pos & 1)) * 16;
-            koffs[i] = (uint32_t)r * (uint32_t)(2 * p.k_rs) + kcol[i];
-            voffs[i] = (uint32_t)r * (uint32_t)(2 * p.v_rs) + vcol[i];
-        }
-    }
-    auto dma = [&](int mt, int buf) {
-#pragma unroll
-        for (int sub = 0; sub < KVM; ++sub) {
-            const int t = mt * KVM + sub;
-            if (KVM > 1 && t >= ktiles) break;
-            char* sK = smem + buf * BUF + sub * TILE;
-            char* sV = sK + K_BYTES;
-            const char* kt = reinterpret_cast<const char*>(kb_ptr + (long)t * 64 * p.k_rs);
-            const char* vt = reinterpret_cast<const char*>(vb_ptr + (long)t * 64 * p.v_rs);
-            const int left = sp.lk - 1 - t * 64;
-            if (left < 63) {
-#pragma unroll
-                for (int i = 0; i < CPW; ++i) {
-                    const uint32_t r = min(drow[i], left);
-                    __builtin_amdgcn_global_load_lds((gptr_t*)(kt + (r * (uint32_t)(2 * p.k_rs) + kcol[i])), (lptr_t*)(sK + (wave * CPW + i) * 1024), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((gptr_t*)(vt + (r * (uint32_t)(2 * p.v_rs) + vcol[i])), (lptr_t*)(sV + (wave * CPW + i) * 1024), 16, 0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < CPW; ++i) {
-                    __builtin_amdgcn_global_load_lds((gptr_t*)(kt + koffs[i]), (lptr_t*)(sK + (wave * CPW + i) * 1024), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((gptr_t*)(vt + voffs[i]), (lptr_t*)(sV + (wave * CPW + i) * 1024), 16, 0, 0);
-                }
-            }
+            const int col = V ? vcol : kcol ^ (D == 64 ? (i * RPC / 2) << 4 : (i * RPC) << 4);
+            uint32_t at = (V ? voff0 : koff0 + col) + (uint32_t)(i * RPC) * (uint32_t)(2 * rs);
+            if (left < 63) at = (uint32_t)min(drow + i * RPC, left) * (uint32_t)(2 * rs) + col;
+            lds_load16(src, at, dst + (wave * CPW + i) * 1024);
         }
     };
     // 8-bit: codes go through registers (16 bytes each), are converted and written as 16-bit tiles: K rows like above, V transposed
@@ -157,46 +164,44 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
     u32x4 k8r[PPT], v8r[PPT];
     uint32_t kbyte[PPT], vbyte[PPT];
-    uint32_t have_next = 0xf, have = 0xf;       // which 16-key groups of the tile have a page
-    // a wave's piece i lies in one 16-key group: one table entry, loaded a tile ahead (lane l: group l & 3), serves its K and its V
-    const int psub = D == 64 ? wave : wave >> 1;
-    int pid = 0;
-    auto look_up = [&](int t) { pid = page_entry(p, b, t * 64 + (lane & 3) * 16); };
-    auto fetch = [&](int t) {
-        have_next = (uint32_t)__ballot(page_ok(p, pid)) & 0xfu;
-        const int pmask = (1 << p.page_shift) - 1;
+    uint32_t have = 0xf, have1 = 0xf, have2 = 0xf;   // which 16-key groups have a page: this tile, the next one, the one after it
+    // a wave's piece i lies in one 16-key group: one table entry (lane l: group l & 3), loaded a tile ahead, serves its K and, a tile
+    // later, its V
+    const int psub = D == 64 ? wave : wave >> 1, pin16 = D == 64 ? lane : (wave & 1) * 64 + lane;   // group of piece i less 2 i; piece of the group
+    int pid_v = 0, pid_k = 0;
+    auto look_up = [&](int t) { return page_entry(p, b, t * 64 + (lane & 3) * 16); };
+    auto groups = [&](int pid) { return (uint32_t)__ballot(page_ok(p, pid)) & 0xfu; };
+    auto fetch = [&](bool V, int t, int pid, u32x4 (&code)[PPT], uint32_t (&byte)[PPT]) {
+#pragma unroll
+        for (int i = 0; i < PPT; ++i) {
+            const int sub = psub + 2 * i, id = __builtin_amdgcn_readlane(pid, sub);
+            const long head = (long)(page_ok(p, id) ? id : 0) * p.Hkv + h;
+            const long at = ((head << p.page_shift) + ((t * 64 + sub * 16) & ((1 << p.page_shift) - 1))) * D + pin16 * 16;
+            byte[i] = (V ? p.v_scale : p.k_scale)[head];
+            code[i] = *reinterpret_cast<const u32x4*>((V ? p.v8 : p.k8) + at);
+        }
+    };
+    auto stage_k = [&](char* sK) {
+#pragma unroll
+        for (int i = 0; i < PPT; ++i) {
+            const int key = (psub + 2 * i) * 16 + pin16 / (D / 16), piece = pin16 % (D / 16), sw = D == 64 ? (key >> 1) & 7 : key & 15;
+            bf16x8 lo, hi;
+            cvt16<FMT>(k8r[i], scale_of(kbyte[i]) * HALF, lo, hi);
+            *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece) ^ sw) * 16) = lo;
+            *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece + 1) ^ sw) * 16) = hi;
+        }
+    };
+    auto stage_v = [&](char* sV) {
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
             const int sub = psub + 2 * i;
-            const int id = __builtin_amdgcn_readlane(pid, sub);
-            const long head = (long)(page_ok(p, id) ? id : 0) * p.Hkv + h;
-            const long at = ((head << p.page_shift) + ((t * 64 + sub * 16) & pmask)) * D;      // of the group's K rows, and of its V
-            const int in = D == 64 ? lane * 16 : ((wave & 1) * 64 + lane) * 16;
-            k8r[i] = *reinterpret_cast<const u32x4*>(p.k8 + at + in);
-            v8r[i] = *reinterpret_cast<const u32x4*>(p.v8 + at + in);
-            kbyte[i] = p.k_scale[head];
-            vbyte[i] = p.v_scale[head];
-        }
-    };
-    auto stage = [&](int buf) {
-        char* sK = smem + buf * BUF;
-        char* sV = sK + K_BYTES;
-#pragma unroll
-        for (int i = 0; i < PPT; ++i) {
-            const int sub = psub + 2 * i, in = D == 64 ? lane : (wave & 1) * 64 + lane;     // 16-byte piece of the group
-            const int key = sub * 16 + in / (D / 16), piece = in % (D / 16), d = in;
             bf16x8 lo, hi;
-            cvt16<FMT>(k8r[i], scale_of(kbyte[i]) * HALF, lo, hi);
-            const int sw = D == 64 ? (key >> 1) & 7 : key & 15;
-            *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece) ^ sw) * 16) = lo;
-            *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece + 1) ^ sw) * 16) = hi;
             cvt16<FMT>(v8r[i], scale_of(vbyte[i]) * HALF, lo, hi);
             const u32x4 a = __builtin_bit_cast(u32x4, lo), z = __builtin_bit_cast(u32x4, hi);
             const u32x4 x = {a[0], a[1], z[0], z[1]}, y = {a[2], a[3], z[2], z[3]};
-            *reinterpret_cast<u32x4*>(sV + swz_off(d, 2 * sub)) = x;
-            *reinterpret_cast<u32x4*>(sV + swz_off(d, 2 * sub + 1)) = y;
+            *reinterpret_cast<u32x4*>(sV + swz_off(pin16, 2 * sub)) = x;
+            *reinterpret_cast<u32x4*>(sV + swz_off(pin16, 2 * sub + 1)) = y;
         }
-        have = have_next;
     };
 
     f32x16 o[QB][NDH];
@@ -236,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
             return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     };
-    auto qk = [&](const char* sK, int qb, f32x16 (&s)[2]) {
+    auto qk = [&](const char* sK, int qb, f32x16 (&s)[2]) __attribute__((always_inline)) {
         const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kvh = 0; kvh < 2; ++kvh)
@@ -246,18 +251,55 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
                 s[kvh] = mfma32h<FMT>(kf, qf[qb][kc], kc == 0 ? zero : s[kvh]);
             }
     };
-    auto sees = [&](int t, int qb, int kvh, int r) {
-        const int key = kvh * 32 + (r & 3) + 8 * (r >> 2) + 4 * fhalf;
-        return t * 64 + key < lim[qb] && (!PAGED || ((have >> (key >> 4)) & 1));
+    // One query block per wave: the operand fragments are read a group of four matrix instructions ahead of their use.  (The LDS reads
+    // and matrix instructions keep this order, other work may move between them: left alone, the compiler reads every fragment right
+    // in front of its use to save registers, and the wave waits for each.)
+    auto order = [&]() { __builtin_amdgcn_sched_barrier(0x0406); };
+    auto qk_ahead = [&](const char* sK, f32x16 (&s)[2]) __attribute__((always_inline)) {
+        const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        bf16x8 f[2][4];
+        auto read = [&](int g, bf16x8 (&x)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const bf16x8*>(sK + (j & 1) * 32 * ROWB + koff[2 * g + (j >> 1)]);
+        };
+        read(0, f[0]);
+#pragma unroll
+        for (int g = 0; g < NKC / 2; ++g) {
+            order();
+            if (g + 1 < NKC / 2) read(g + 1, f[(g + 1) & 1]);
+            order();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j & 1] = mfma32h<FMT>(f[g & 1][j], qf[0][2 * g + (j >> 1)], g == 0 && j < 2 ? zero : s[j & 1]);
+        }
+        order();
     };
-    auto mask = [&](int t, int qb, f32x16 (&s)[2]) {
+    auto pv_ahead = [&](const char* sV, const bf16x8 (&pf)[2][2]) __attribute__((always_inline)) {
+        bf16x8 f[2][NDH];
+        auto read = [&](int g, bf16x8 (&x)[NDH]) {
+#pragma unroll
+            for (int dh = 0; dh < NDH; ++dh) x[dh] = v_frag(sV, g >> 1, g & 1, dh);
+        };
+        read(0, f[0]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            order();
+            if (g < 3) read(g + 1, f[(g + 1) & 1]);
+            order();
+#pragma unroll
+            for (int dh = 0; dh < NDH; ++dh) o[0][dh] = mfma32h<FMT>(f[g & 1][dh], pf[g >> 1][g & 1], o[0][dh]);
+        }
+        order();
+    };
+    auto mask = [&](int t, int qb, f32x16 (&s)[2], uint32_t groups_) __attribute__((always_inline)) {
+        asm volatile("");                                  // (keeps the branch: as selects this would be half of every tile's work)
+        const int seen = lim[qb] - t * 64 - 4 * fhalf;     // key kvh * 32 + (r & 3) + 8 (r >> 2) (+ 4 half) is seen if it is less
 #pragma unroll
         for (int kvh = 0; kvh < 2; ++kvh)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (!sees(t, qb, kvh, r)) s[kvh][r] = -INFINITY;
+                if (kvh * 32 + (r & 3) + 8 * (r >> 2) >= seen || (PAGED && !((groups_ >> (kvh * 2 + (r >> 3))) & 1))) s[kvh][r] = -INFINITY;
     };
-    auto update_max = [&](int qb, const f32x16 (&s)[2]) {
+    auto row_max = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
         float mx = s[0][0];
 #pragma unroll
         for (int kvh = 0; kvh < 2; ++kvh)
@@ -265,7 +307,9 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kvh][r]);
         const uint32_t bits = __builtin_bit_cast(uint32_t, mx);
         const auto sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
-        mx = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1])) * c;
+        return fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1])) * c;
+    };
+    auto raise_max = [&](int qb, float mx) __attribute__((always_inline)) {
         if (__any(mx > m_run[qb] + DEFER_THR)) {
             const float m_new = fmaxf(m_run[qb], mx);
             const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
@@ -277,7 +321,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
                 for (int r = 0; r < 16; ++r) o[qb][dh][r] *= alpha;
         }
     };
-    auto exp_pack = [&](int qb, f32x16 (&s)[2], bf16x8 (&pf)[2][2]) {
+    auto exp_pack = [&](int qb, f32x16 (&s)[2], bf16x8 (&pf)[2][2]) __attribute__((always_inline)) {
         const float m = m_run[qb] - (FMT == FMT_F16 ? P_SHIFT_F16 : 0.f);
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -308,16 +352,18 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         else
             return key * ROWB + (D == 64 ? ((d >> 4) ^ (key & 2)) << 5 : ((d >> 4) ^ ((key & 3) << 1)) << 5) + 2 * (d & 15);
     };
-    // a tile whose V holds inf or NaN (workgroup-uniform): advance the maxima first, so that no later rescale of this tile meets
-    // the infinities; add them to the rows that see them; leave zeros for the matrix product
-    auto absorb_nonfinite = [&](char* sK, char* sV, int t) {
+    // a tile whose V holds inf or NaN (workgroup-uniform): with the maxima raised to the tile's, so that its rescale does not meet the
+    // infinities, add them to the rows that see them and leave zeros for the matrix product
+    auto absorb_nonfinite = [&](char* sK, char* sV, int t) __attribute__((always_inline)) {
         if (t * 64 < w_last) {
+            if constexpr (QB == 2) {
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-                f32x16 s[2];
-                qk(sK, qb, s);
-                mask(t, qb, s);
-                update_max(qb, s);
+                for (int qb = 0; qb < QB; ++qb) {
+                    f32x16 s[2];
+                    qk(sK, qb, s);
+                    mask(t, qb, s, 0xf);
+                    raise_max(qb, row_max(s));
+                }
             }
 #pragma unroll 1
             for (int key = 0; key < 64; ++key) {
@@ -349,7 +395,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         __syncthreads();
     };
 
-    // keeps the packed numerators of the first query block where they are formed, beside the second block's score products
+    // keeps packed numerators where they are formed, beside the score products in the same block of instructions
     auto pin = [&](bf16x8 (&pf)[2][2]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -359,59 +405,147 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         }
     };
 
-    if (t0 < t1) {
-        if constexpr (PAGED) {
-            look_up(t0);
-            fetch(t0);
-            look_up(t0 + 1);
-            stage(t0 & 1);
-        } else {
-            dma(t0, t0 & 1);
-        }
-        __syncthreads();   // (drains the DMA as well)
-        for (int mt = t0; mt < t1; ++mt) {
+    auto tile_nonfinite = [&](const char* sV) __attribute__((always_inline)) {
+        bool bad = false;
+        for (int i = tid * 16; i < K_BYTES; i += 4096) bad = bad || nonfinite8<FMT>(*reinterpret_cast<const bf16x8*>(sV + i));
+        return __syncthreads_or(bad) != 0;
+    };
+
+    if constexpr (QB == 1) {
+        // One query block per wave, pipelined over the tiles: the score product of tile t + 1 runs beside the exponentials of tile t, the
+        // maximum of t + 1 beside the second product of t (LDS holds K of t + 1 and V of t while K of t + 2 and V of t + 1 arrive).
+        auto kbuf = [&](int t) { return smem + (t & 1) * K_BYTES; };
+        auto vbuf = [&](int t) { return smem + (2 + (t & 1)) * K_BYTES; };
+        auto step = [&](int t, f32x16 (&s)[2], f32x16 (&sn)[2], char* k_next, char* v_here, char* k_dst, char* v_dst) __attribute__((always_inline)) {
             if constexpr (PAGED) {
-                // (the last tile fetches itself again: a branch here would make every wait one for all loads)
-                fetch(min(mt + 1, t1 - 1));
-                look_up(mt + 2);
+                // (past the last tile it is fetched again: a branch here would make every later wait one for all loads)
+                const int tk = min(t + 2, t1 - 1);
+                fetch(true, t + 1, pid_v, v8r, vbyte);
+                fetch(false, tk, pid_k, k8r, kbyte);
+                have2 = groups(pid_k);
+                pid_v = pid_k;
+                pid_k = look_up(min(t + 3, t1 - 1));
             } else {
-                if (mt + 1 < t1) dma(mt + 1, (mt + 1) & 1);
+                dma(true, t + 1, v_dst);
+                if (t + 2 < t1) dma(false, t + 2, k_dst);
             }
+            if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
+                if (tile_nonfinite(v_here)) absorb_nonfinite(nullptr, v_here, t);
+            }
+            if (t * 64 < w_last) {
+                // (behind a wave's last key the score product runs on what the buffer holds and is dropped: as a branch it would take the
+                // exponentials out of the block of instructions in which they run beside it)
+                const bool more = (t + 1) * 64 < w_last;
+                bf16x8 pf[2][2];
+                qk_ahead(k_next, sn);
+                exp_pack(0, s, pf);
+                pin(pf);
+                if (more && ((t + 2) * 64 > w_first || (PAGED && have1 != 0xf))) mask(t + 1, 0, sn, have1);
+                pv_ahead(v_here, pf);
+                const float mx = row_max(sn);
+                raise_max(0, more ? mx : M_INIT);
+            }
+            if constexpr (PAGED) {
+                stage_v(v_dst);
+                stage_k(k_dst);
+                have = have1;
+                have1 = have2;
+            }
+            arrive();
+        };
+        if (t0 < t1) {
+            const int t2 = min(t0 + 1, t1 - 1);
+            if constexpr (PAGED) {
+                const int pid = look_up(t0);
+                pid_v = look_up(t2);
+                pid_k = look_up(min(t0 + 2, t1 - 1));
+                have = groups(pid);
+                have1 = groups(pid_v);
+                fetch(false, t0, pid, k8r, kbyte);
+                fetch(true, t0, pid, v8r, vbyte);
+                stage_k(kbuf(t0));
+                stage_v(vbuf(t0));
+                fetch(false, t2, pid_v, k8r, kbyte);
+                if (t2 != t0) stage_k(kbuf(t2));
+            } else {
+                dma(false, t0, kbuf(t0));
+                dma(true, t0, vbuf(t0));
+                if (t2 != t0) dma(false, t2, kbuf(t2));
+            }
+            f32x16 sa[2], sb[2];
+            arrive();
+            if (t0 * 64 < w_last) {
+                qk(kbuf(t0), 0, sa);
+                if ((t0 + 1) * 64 > w_first || (PAGED && have != 0xf)) mask(t0, 0, sa, have);
+                raise_max(0, row_max(sa));
+            }
+            if (t1 - t0 > 2) __syncthreads();   // (the first step loads over the tile just read)
+            for (int t = t0; t + 1 < t1; t += 2) {
+                step(t, sa, sb, kbuf(t + 1), vbuf(t), kbuf(t), vbuf(t + 1));
+                if (t + 2 < t1) {
+                    step(t + 1, sb, sa, kbuf(t), vbuf(t + 1), kbuf(t + 1), vbuf(t));
+                } else {
+                    sa[0] = sb[0];
+                    sa[1] = sb[1];
+                }
+            }
+            // the last tile has no score product beside it
+            char* sV = vbuf(t1 - 1);
+            if (t1 * 64 > wg_first || (PAGED && have != 0xf)) {
+                if (tile_nonfinite(sV)) absorb_nonfinite(nullptr, sV, t1 - 1);
+            }
+            if ((t1 - 1) * 64 < w_last) {
+                bf16x8 pf[2][2];
+                exp_pack(0, sa, pf);
+                pv_ahead(sV, pf);
+            }
+        }
+    } else {
+        // Two query blocks per wave, offset against each other within the tile: the score product of the second runs beside the
+        // exponentials of the first, the second product of the first beside the exponentials of the second.
+        static_assert(QB == 1 || !PAGED, "paged tiles have one query block");
+        auto load = [&](int mt, char* dst) {
 #pragma unroll
             for (int sub = 0; sub < KVM; ++sub) {
                 const int t = mt * KVM + sub;
-                if (KVM > 1 && t >= ktiles) break;
-                char* sK = smem + (mt & 1) * BUF + sub * TILE;
+                if (t >= ktiles) break;
+                dma(false, t, dst + sub * TILE);
+                dma(true, t, dst + sub * TILE + K_BYTES);
+            }
+        };
+        auto step = [&](int mt, char* here, char* dst) {
+            if (mt + 1 < t1) load(mt + 1, dst);
+#pragma unroll
+            for (int sub = 0; sub < KVM; ++sub) {
+                const int t = mt * KVM + sub;
+                if (t >= ktiles) break;
+                char* sK = here + sub * TILE;
                 char* sV = sK + K_BYTES;
-                if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
-                    bool bad = false;
-                    for (int i = tid * 16; i < K_BYTES; i += 4096) bad = bad || nonfinite8<FMT>(*reinterpret_cast<const bf16x8*>(sV + i));
-                    if (__syncthreads_or(bad)) absorb_nonfinite(sK, sV, t);
+                if ((t + 1) * 64 > wg_first) {
+                    if (tile_nonfinite(sV)) absorb_nonfinite(sK, sV, t);
                 }
                 if (t * 64 >= w_last) continue;
-                const bool edge = (t + 1) * 64 > w_first || (PAGED && have != 0xf);
+                const bool edge = (t + 1) * 64 > w_first;
                 f32x16 s0[2], s1[2];
                 bf16x8 pf0[2][2], pf1[2][2];
                 qk(sK, 0, s0);
-                if (edge) mask(t, 0, s0);
-                update_max(0, s0);
-                if constexpr (QB == 2) qk(sK, 1, s1);
+                if (edge) mask(t, 0, s0, 0xf);
+                raise_max(0, row_max(s0));
+                qk(sK, QB - 1, s1);
                 exp_pack(0, s0, pf0);
-                if constexpr (QB == 2) {
-                    pin(pf0);
-                    if (edge) mask(t, 1, s1);
-                    update_max(1, s1);
-                }
+                pin(pf0);
+                if (edge) mask(t, QB - 1, s1, 0xf);
+                raise_max(QB - 1, row_max(s1));
                 pv(sV, 0, pf0);
-                if constexpr (QB == 2) {
-                    exp_pack(1, s1, pf1);
-                    pv(sV, 1, pf1);
-                }
+                exp_pack(QB - 1, s1, pf1);
+                pv(sV, QB - 1, pf1);
             }
-            if constexpr (PAGED) {
-                if (mt + 1 < t1) stage((mt + 1) & 1);
-            }
-            __syncthreads();
+            arrive();
+        };
+        if (t0 < t1) {
+            load(t0, smem + (t0 & 1) * BUF);
+            arrive();
+            for (int mt = t0; mt < t1; ++mt) step(mt, smem + (mt & 1) * BUF, smem + (1 - (mt & 1)) * BUF);
         }
     }
 
@@ -467,8 +601,8 @@ int launch(const SeqAttnParams& p_in, hipStream_t stream) {
 template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
     if (D == 128) return launch<128, 1, 1, FMT, PAGED>(p, stream);
-    constexpr int KVM = PAGED ? 1 : 2;
-    return small ? launch<64, 1, KVM, FMT, PAGED>(p, stream) : launch<64, 2, KVM, FMT, PAGED>(p, stream);
+    if constexpr (PAGED) return launch<64, 1, 1, FMT, PAGED>(p, stream);
+    else return small ? launch<64, 1, 1, FMT, PAGED>(p, stream) : launch<64, 2, 2, FMT, PAGED>(p, stream);
 }
 
 }  // namespace
@@ -478,21 +612,29 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
     return paged ? launch_fmt<FMT_BF16, true>(p, D, small, stream) : launch_fmt<FMT_BF16, false>(p, D, small, stream);
 }
 
-SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D) {
+// Key ranges of a grid of `items` tiles that does not fill the chip.  With n = ceil(items s / 256) work items on the fullest CU, each
+// 1 / s of a tile's keys, it is done after n / (s e(n)); a CU reaches about 0.55, 0.85 and all of its rate with one, two and three
+// resident work items.  The fold moves 8 D bytes per row and range, 240 s / keys of the tiles' own time at the rates of this card.
+SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D, bool paged) {
     SeqPlan plan = {};
-    const long rows = max_q * G, pairs = (long)B * Hkv, slots = 512;   // two workgroups on each of 256 CUs
-    plan.small = D == 64 && (rows <= 128 || pairs * ((rows + 255) / 256) < slots);
+    const long rows = max_q * G, pairs = (long)B * Hkv, cus = 256;
+    plan.small = D == 64 && (paged || rows <= 128 || pairs * ((rows + 255) / 256) < 2 * cus);
     const int bm = (D == 128 || plan.small) ? 128 : 256;
     const long items = pairs * ((rows + bm - 1) / bm);
-    long s = 1;
-    if (items < slots) {
-        s = slots / (items < 1 ? 1 : items);
-        const long most = max_k / 512;      // at least eight tiles per range
-        if (s > most) s = most;
-        if (s > 32) s = 32;
-        if (s < 1) s = 1;
+    plan.splits = 1;
+    if (items < 3 * cus && max_k >= 1024) {
+        const long most = max_k / 512 < 32 ? max_k / 512 : 32;      // at least eight tiles per range
+        double best = 1e30;
+        for (long s = 1; s <= most; ++s) {
+            const long n = (items * s + cus - 1) / cus;
+            const double rate = n == 1 ? 0.55 : n == 2 ? 0.85 : 1.0;
+            const double cost = (double)n / (s * rate) + (s > 1 ? (double)items / cus * 240.0 * s / max_k : 0.0);
+            if (cost < best * 0.97) {
+                best = cost;
+                plan.splits = (int)s;
+            }
+        }
     }
-    plan.splits = (int)s;
     return plan;
 }
 
@@ -513,7 +655,7 @@ static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const v
     p.cu_q = cu_q; p.cu_k = cu_k;
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.Tq = Tq; p.Tk = Tk; p.max_q = max_q; p.causal = causal != 0;
     p.scale_log2 = scale * 1.4426950408889634f;
-    const SeqPlan plan = iggt_seq_tile_plan(B, max_q, max_k, Hkv, p.G, D);
+    const SeqPlan plan = iggt_seq_tile_plan(B, max_q, max_k, Hkv, p.G, D, false);
     p.splits = plan.splits;
     if (p.splits > 1) {
         const long n = (long)p.splits * B * max_q * Hq;
@@ -529,7 +671,7 @@ static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const v
 extern "C" {
 long iggt_packed_attn_ws_bytes(int B, int max_q, int max_k, int Hq, int Hkv, int D) {
     if (B <= 0 || max_q <= 0 || max_k < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return 0;
-    const SeqPlan plan = iggt_seq_tile_plan(B, max_q, max_k, Hkv, Hq / Hkv, D);
+    const SeqPlan plan = iggt_seq_tile_plan(B, max_q, max_k, Hkv, Hq / Hkv, D, false);
     return plan.splits > 1 ? (long)plan.splits * B * max_q * Hq * (D + 2) * 4 : 0;
 }
 int iggt_packed_attn_bf16(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs,

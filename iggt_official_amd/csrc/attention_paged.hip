@@ -353,14 +353,20 @@ int launch_rows(const SeqAttnParams& p, int fmt, hipStream_t stream) {
 // Up to 16 rows per (request, key head): the row kernel.  Its key ranges are of one length, a multiple of 256 keys, whatever the
 // requests' own lengths, so that requests of different lengths fill the chip evenly; the range is as long as leaves about 2 500
 // work items (three to five rounds of the chip) if all requests had max_len tokens, and FOLD_MAX ranges at most.
+// Short requests are not split: the fold is a second launch (3.4 us, and as much again of the host's time), a wave's 64 keys are
+// 0.5 us (D = 64) or 0.9 us (128).  Measured, split / not: 1 x 16 heads of 64, 1 374 tokens 8.2 / 7.3 us, 2 048 8.1 / 8.8 (in a loop of
+// calls 12.9 / 9.5), 4 096 8.6 / 12.8; 4 heads of 128, 1 374 tokens 9.7 / 10.7 (12.8 / 10.8), 2 048 9.7 / 13.3.  Pairs that fill the chip
+// gain longer: 16 x 16 heads of 64, 4 096 tokens 25.6 / 21.6.
 bool few_rows(long max_q, int G) { return max_q * G <= 16; }
 SeqPlan paged_plan(int B, long max_q, long max_len, int Hkv, int G, int D) {
-    if (!few_rows(max_q, G)) return iggt_seq_tile_plan(B, max_q, max_len, Hkv, G, D);
+    if (!few_rows(max_q, G)) return iggt_seq_tile_plan(B, max_q, max_len, Hkv, G, D, true);
     const long pairs = (long)B * Hkv, blocks = (max_len + 63) / 64;
     long want = 2560 / pairs;
     if (want > FOLD_MAX) want = FOLD_MAX;
     if (want < 1) want = 1;
     long range = ((blocks + want - 1) / want + 3) / 4 * 4;
+    const long single = pairs >= 256 ? 64 : (D == 64 ? 32 : 24);
+    if (blocks <= single) range = (blocks + 3) / 4 * 4;
     if (range < 4) range = 4;
     SeqPlan plan = {(int)((blocks + range - 1) / range), false, (int)range};
     if (plan.splits < 1) plan.splits = 1;

@@ -132,4 +132,4 @@ struct SeqPlan {
     bool small;   // 128-row tiles where 256-row ones exist
     int range_blocks;
 };
-SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D);
+SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D, bool paged);
