@@ -612,9 +612,9 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
     return paged ? launch_fmt<FMT_BF16, true>(p, D, small, stream) : launch_fmt<FMT_BF16, false>(p, D, small, stream);
 }
 
-// Key ranges of a grid of `items` tiles that does not fill the chip.  With n = ceil(items s / 256) work items on the fullest CU, each
-// 1 / s of a tile's keys, it is done after n / (s e(n)); a CU reaches about 0.55, 0.85 and all of its rate with one, two and three
-// resident work items.  The fold moves 8 D bytes per row and range, 240 s / keys of the tiles' own time at the rates of this card.
+// Key ranges of a grid of `items` tiles that does not fill the chip.  The fullest CU has n = ceil(items s / 256) work items, each 1 / s of
+// a tile's keys; it runs them two at a time, and one alone at about 0.55 of the rate.  The fold moves 8 D bytes per row and range,
+// 240 s / keys of the tiles' own time at the rates of this card.
 SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D, bool paged) {
     SeqPlan plan = {};
     const long rows = max_q * G, pairs = (long)B * Hkv, cus = 256;
@@ -622,13 +622,12 @@ SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D,
     const int bm = (D == 128 || plan.small) ? 128 : 256;
     const long items = pairs * ((rows + bm - 1) / bm);
     plan.splits = 1;
-    if (items < 3 * cus && max_k >= 1024) {
+    if (items < 4 * cus && max_k >= 1024) {
         const long most = max_k / 512 < 32 ? max_k / 512 : 32;      // at least eight tiles per range
         double best = 1e30;
         for (long s = 1; s <= most; ++s) {
             const long n = (items * s + cus - 1) / cus;
-            const double rate = n == 1 ? 0.55 : n == 2 ? 0.85 : 1.0;
-            const double cost = (double)n / (s * rate) + (s > 1 ? (double)items / cus * 240.0 * s / max_k : 0.0);
+            const double cost = ((double)(n / 2 * 2) + (n % 2) / 0.55) / s + (s > 1 ? (double)items / cus * 240.0 * s / max_k : 0.0);
             if (cost < best * 0.97) {
                 best = cost;
                 plan.splits = (int)s;

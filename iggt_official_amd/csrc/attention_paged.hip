@@ -324,11 +324,54 @@ __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams 
     }
 }
 
+// The same for up to 8 ranges: a thread folds four channels of a row by itself, all its loads independent.
+template <int D, int FMT, bool PAGED>
+__global__ __launch_bounds__(256) void seq_attn_fold_few_kernel(const SeqAttnParams p) {
+    constexpr int LPR = D / 4;
+    constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
+    const int d = (int)(threadIdx.x % LPR) * 4;
+    const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;    // ((b, token), head)
+    const long per = (long)p.max_q * p.Hq;
+    const int b = (int)(row / per);
+    if (b >= p.B) return;
+    const SeqSpan sp = seq_span<PAGED>(p, b);
+    const int i = (int)((row - b * per) / p.Hq), hq = (int)(row % p.Hq);
+    if (i >= sp.lq) return;
+    const long step = (long)p.B * per;
+    float m[8], l[8], top = M_INIT;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        m[s] = M_INIT;
+        l[s] = 0.f;
+        if (s < p.splits) {
+            m[s] = p.part_ml[2 * (s * step + row)];
+            l[s] = p.part_ml[2 * (s * step + row) + 1];
+        }
+        top = fmaxf(top, m[s]);
+    }
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        if (s < p.splits && l[s] != 0.f) {
+            const float f = __builtin_amdgcn_exp2f(m[s] - top);
+            total += l[s] * f;
+            acc += *reinterpret_cast<const f32x4*>(p.part_o + (s * step + row) * D + d) * f;
+        }
+    }
+    const float inv = total == 0.f ? 0.f : (1.0f / HALF) / total;
+    u32x2 w;
+    w[0] = pack_h2<FMT, false>(acc[0] * inv, acc[1] * inv);
+    w[1] = pack_h2<FMT, false>(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<u32x2*>(p.o + (long)(sp.q0 + i) * p.o_rs + (long)hq * p.o_hs + d) = w;
+}
+
 template <int D, int FMT, bool PAGED>
 int launch_fold(const SeqAttnParams& p, hipStream_t stream) {
     const long rows = (long)p.B * p.max_q * p.Hq;
     if (rows >= (1L << 31)) return -4;
-    if (rows <= 2048) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT, PAGED, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p);
+    if (p.splits <= 8) hipLaunchKernelGGL((seq_attn_fold_few_kernel<D, FMT, PAGED>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, stream, p);
+    else if (rows <= 2048) hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT, PAGED, 4>), dim3((unsigned)rows), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((seq_attn_fold_kernel<D, FMT, PAGED, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
