@@ -204,15 +204,34 @@ IGGT_DEVINL void write_run(const AppendParams& p, int t0, int len, int page, int
     uint8_t* dst = (V ? p.v8 : p.k8) + ((head << p.shift) * D);
     constexpr int LPR = D / 8, RPI = 64 / LPR;   // lanes of a row (8 values each), rows of one load
     const int lr = lane / LPR, lc = (lane % LPR) * 8;
-    float m = 0.f;
-    for (int i = lr; i < len; i += RPI) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(src + (long)i * rs + lc);
+    // U loads in flight at a time; K of a run that fits into them is not read again
+    constexpr int U = 4;
+    u32x4 x[U];
+    auto read = [&](int from) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = amax2<FMT>(m, w[j]);
+        for (int j = 0; j < U; ++j) {
+            const int i = from + j * RPI + lr;
+            x[j] = i < len ? *reinterpret_cast<const u32x4*>(src + (long)i * rs + lc) : u32x4{0u, 0u, 0u, 0u};
+        }
+    };
+    const int held = at > 0 ? (int)*scale : 0;
+    float m = 0.f;
+    if (len <= RPI) {    // a token, or a few: one load
+        x[0] = lr < len ? *reinterpret_cast<const u32x4*>(src + (long)lr * rs + lc) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m = amax2<FMT>(m, x[0][q]);
+    } else {
+        for (int from = 0; from < len; from += U * RPI) {
+            read(from);
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) m = amax2<FMT>(m, x[j][q]);
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const int need = scale_byte(m), old = at > 0 ? (int)*scale : 0, now = max(old, need);
+    const int need = scale_byte(m), old = held, now = max(old, need);
     // 2^(127 - now): the last two exponents have a subnormal reciprocal (2^-127)
     const float inv = now >= 254 ? __builtin_bit_cast(float, 0x00400000u) : pow2_byte(254 - now);
     const bool moved = at > 0 && now > old;
@@ -226,13 +245,18 @@ IGGT_DEVINL void write_run(const AppendParams& p, int t0, int len, int page, int
                 for (int j = 0; j < 4; ++j) w[j] = scale4(w[j], down);
                 reinterpret_cast<u32x4*>(dst)[i] = w;
             }
-        for (int i = lr; i < len; i += RPI) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(src + (long)i * rs + lc);
-            u32x2 c;
+        for (int from = 0; from < len; from += U * RPI) {
+            if (len > U * RPI) read(from);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                c[j] = code4(h2_lo<FMT>(w[2 * j]) * inv, h2_hi<FMT>(w[2 * j]) * inv, h2_lo<FMT>(w[2 * j + 1]) * inv, h2_hi<FMT>(w[2 * j + 1]) * inv);
-            *reinterpret_cast<u32x2*>(dst + (long)(at + i) * D + lc) = c;
+            for (int j = 0; j < U; ++j) {
+                const int i = from + j * RPI + lr;
+                if (i >= len) break;
+                u32x2 c;
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    c[q] = code4(h2_lo<FMT>(x[j][2 * q]) * inv, h2_hi<FMT>(x[j][2 * q]) * inv, h2_lo<FMT>(x[j][2 * q + 1]) * inv, h2_hi<FMT>(x[j][2 * q + 1]) * inv);
+                *reinterpret_cast<u32x2*>(dst + (long)(at + i) * D + lc) = c;
+            }
         }
     } else {
         // 16 tokens of a channel pair per lane: D / 2 lanes per group of 16 tokens
@@ -248,17 +272,17 @@ IGGT_DEVINL void write_run(const AppendParams& p, int t0, int len, int page, int
                 c[0] = *reinterpret_cast<const u32x4*>(out);
                 c[1] = *reinterpret_cast<const u32x4*>(out + 16);
             }
-            uint32_t x[16];
+            uint32_t y[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const int i = first + j;
-                x[j] = (i >= 0 && i < len) ? *reinterpret_cast<const uint32_t*>(src + (long)i * rs + d) : 0u;
+                y[j] = (i >= 0 && i < len) ? *reinterpret_cast<const uint32_t*>(src + (long)i * rs + d) : 0u;
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t nw[2];
-                nw[0] = code4(h2_lo<FMT>(x[4 * q]) * inv, h2_lo<FMT>(x[4 * q + 1]) * inv, h2_lo<FMT>(x[4 * q + 2]) * inv, h2_lo<FMT>(x[4 * q + 3]) * inv);
-                nw[1] = code4(h2_hi<FMT>(x[4 * q]) * inv, h2_hi<FMT>(x[4 * q + 1]) * inv, h2_hi<FMT>(x[4 * q + 2]) * inv, h2_hi<FMT>(x[4 * q + 3]) * inv);
+                nw[0] = code4(h2_lo<FMT>(y[4 * q]) * inv, h2_lo<FMT>(y[4 * q + 1]) * inv, h2_lo<FMT>(y[4 * q + 2]) * inv, h2_lo<FMT>(y[4 * q + 3]) * inv);
+                nw[1] = code4(h2_hi<FMT>(y[4 * q]) * inv, h2_hi<FMT>(y[4 * q + 1]) * inv, h2_hi<FMT>(y[4 * q + 2]) * inv, h2_hi<FMT>(y[4 * q + 3]) * inv);
                 if (whole) {
                     c[0][q] = nw[0];
                     c[1][q] = nw[1];
@@ -291,26 +315,24 @@ __global__ __launch_bounds__(256) void append_pages_kernel(const AppendParams p,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.y * 2 + (wave >> 1);
     if (h >= p.Hkv) return;
-    const int psize = 1 << p.shift;
-    const int a = blockIdx.x * group, z = min(a + group, p.T);
+    const int psize = 1 << p.shift, lane = threadIdx.x & 63;
+    const int a = blockIdx.x * group;
     auto slot_at = [&](int t) {
-        const int s = p.slots[t];
+        const int s = (t >= 0 && t < p.T) ? p.slots[t] : -1;
         return (unsigned)s < (unsigned)p.num_slots ? s : -1;
     };
-    int before = a > 0 ? slot_at(a - 1) : -1;
-    for (int t = a; t < z;) {
-        const int s = slot_at(t);
-        const bool begins = s >= 0 && (before < 0 || before != s - 1 || (s & (psize - 1)) == 0);
-        before = s;
-        if (!begins) {
-            ++t;
-            continue;
-        }
-        // length of the run: a wave looks at 64 following slots at a time
-        const int at = s & (psize - 1), most = min(psize - at, p.T - t);
-        int len = 0;
-        while (len < most) {
-            const int i = len + (int)(threadIdx.x & 63);
+    // lane l looks at token a + l: does a run begin there
+    const int mine = slot_at(a + lane), before = slot_at(a + lane - 1);
+    unsigned long long begins = __ballot(lane < group && mine >= 0 && (before < 0 || before != mine - 1 || (mine & (psize - 1)) == 0));
+    while (begins != 0) {
+        const int l = __builtin_ctzll(begins), t = a + l;
+        begins &= begins - 1;
+        const int s = __builtin_amdgcn_readlane(mine, l), at = s & (psize - 1), most = min(psize - at, p.T - t);
+        // length of the run: among the 64 slots at hand, and only if it goes on behind them 64 more at a time
+        const unsigned long long goes_on = __ballot(mine == s + (lane - l)) >> l;
+        int len = min(goes_on == ~0ull ? 64 : __builtin_ctzll(~goes_on), most);
+        while (len >= 64 - l && len < most) {
+            const int i = len + lane;
             const unsigned long long same = __ballot(i < most && p.slots[t + (i < most ? i : 0)] == s + i);
             const int run = same == ~0ull ? 64 : __builtin_ctzll(~same);
             len += run;
@@ -318,8 +340,6 @@ __global__ __launch_bounds__(256) void append_pages_kernel(const AppendParams p,
         }
         if (wave & 1) write_run<D, FMT, true>(p, t, len, s >> p.shift, at, h);
         else write_run<D, FMT, false>(p, t, len, s >> p.shift, at, h);
-        t += len;
-        before = s + len - 1;
     }
 }
 
@@ -332,9 +352,10 @@ int append_h16(int fmt, const void* k, long k_rs, long k_hs, const void* v, long
     if (T == 0 || num_pages == 0) return 0;
     AppendParams p = {(const uint16_t*)k, (const uint16_t*)v, k_rs, k_hs, v_rs, v_hs, slots, T, Hkv, num_pages << shift, shift,
                       (uint8_t*)k_codes, (uint8_t*)v_codes, (uint8_t*)k_scale, (uint8_t*)v_scale};
-    // Single tokens of many requests are all runs of their own: one workgroup for each.  A long prompt has a run per page: groups
-    // of 16 tokens, of which most find no beginning, keep the number of workgroups down.
-    const int group = (long)T * Hkv <= 16384 ? 1 : 16;
+    // Single tokens of many requests are all runs of their own: a workgroup each.  A prompt has a run per page: groups as long as leave
+    // about four workgroups per CU.
+    const long heads2 = (Hkv + 1) / 2;
+    const int group = (long)T / 64 * heads2 >= 1024 ? 64 : ((long)T / 16 * heads2 >= 256 ? 16 : 1);
     const dim3 grid((T + group - 1) / group, (Hkv + 1) / 2), block(256);
     const hipStream_t st = (hipStream_t)stream;
     if (fmt == FMT_F16) {
