@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int PLAN_MAX_REQUESTS = 8192, PLAN_THREADS = 1024;
+constexpr int PLAN_MAX_REQUESTS = 8192, PLAN_THREADS = 512, PLAN_WAVES = PLAN_THREADS / 64;
 
 struct PlanParams {
     int* tables;
@@ -54,8 +54,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_pages_kernel(const PlanPara
     int* s_tok = lds;                 // exclusive prefix sums over the requests: tokens,
     int* s_grow = lds + p.R;          // pages taken,
     int* s_shrink = lds + 2 * p.R;    // pages given back
-    __shared__ int s_wave[3][16];
-    __shared__ long s_total[3][16];
+    int* s_have = lds + 3 * p.R;      // tokens held
+    __shared__ int s_wave[3][PLAN_WAVES];
+    __shared__ long s_total[3][PLAN_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int cap = p.M << p.shift, round = (1 << p.shift) - 1;
     const int N = p.N;
@@ -65,17 +66,30 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_pages_kernel(const PlanPara
     const int per = (p.R + PLAN_THREADS - 1) / PLAN_THREADS, r0 = tid * per, r1 = min(r0 + per, p.R);
     int sum[3] = {0, 0, 0};
     long total[3] = {0, 0, 0};        // 64 bits: lengths are whatever the caller's memory holds
-    for (int r = r0; r < r1; ++r) {
-        const int have = min(max(p.lens[r], 0), cap), want = min(max(p.new_lens[r], 0), cap);
-        const int hp = (have + round) >> p.shift, wp = (want + round) >> p.shift;
-        const int v[3] = {max(want - have, 0), max(wp - hp, 0), max(hp - wp, 0)};
-        s_tok[r] = sum[0];
-        s_grow[r] = sum[1];
-        s_shrink[r] = sum[2];
+    for (int r = r0; r < r1; r += 4) {
+        int have[4], want[4];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            sum[i] = (int)((unsigned)sum[i] + (unsigned)v[i]);
-            total[i] += v[i];
+        for (int j = 0; j < 4; ++j) {
+            const int q = min(r + j, r1 - 1);
+            have[j] = p.lens[q];
+            want[j] = p.new_lens[q];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (r + j >= r1) break;
+            have[j] = min(max(have[j], 0), cap);
+            want[j] = min(max(want[j], 0), cap);
+            const int hp = (have[j] + round) >> p.shift, wp = (want[j] + round) >> p.shift;
+            const int v[3] = {max(want[j] - have[j], 0), max(wp - hp, 0), max(hp - wp, 0)};
+            s_tok[r + j] = sum[0];
+            s_grow[r + j] = sum[1];
+            s_shrink[r + j] = sum[2];
+            s_have[r + j] = have[j];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                sum[i] = (int)((unsigned)sum[i] + (unsigned)v[i]);
+                total[i] += v[i];
+            }
         }
     }
     int incl[3];
@@ -97,7 +111,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_pages_kernel(const PlanPara
     __syncthreads();
     long all[3] = {0, 0, 0};
     unsigned base[3] = {0, 0, 0};
-    for (int w = 0; w < PLAN_THREADS / 64; ++w)
+#pragma unroll
+    for (int w = 0; w < PLAN_WAVES; ++w)
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             all[i] += s_total[i][w];
@@ -115,25 +130,25 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_pages_kernel(const PlanPara
 
     if (blockIdx.x == 0) {
         for (int r = tid; r < p.R; r += PLAN_THREADS) {
-            const int have = min(max(p.lens[r], 0), cap), want = min(max(p.new_lens[r], 0), cap);
+            const int have = s_have[r], want = min(max(p.new_lens[r], 0), cap);
             p.starts[r] = fits ? s_tok[r] : 0;
             p.next_lens[r] = fits ? want : min(have, want);
         }
         if (tid == 0) {
             p.starts[p.R] = ntok;
-            p.next_counters[0] = N > 0 ? (int)(((long)head + ngrow) % N) : 0;
+            p.next_counters[0] = N > 0 ? (int)(((unsigned)head + (unsigned)ngrow) % (unsigned)N) : 0;
             p.next_counters[1] = count - ngrow + nshrink;
             p.next_counters[2] = all[0] > p.T ? -1 : (all[1] > count ? (int)min(all[1] - count, (long)0x7fffffff) : 0);
         }
     }
     const int gtid = blockIdx.x * PLAN_THREADS + tid, gsize = gridDim.x * PLAN_THREADS;
-    auto taken = [&](int i) { return p.ring[((long)head + i) % N]; };
+    auto wrap = [&](unsigned i) { return i >= (unsigned)N ? i - (unsigned)N : i; };    // of i < 2 N
+    auto taken = [&](int i) { return p.ring[wrap((unsigned)head + (unsigned)i)]; };     // i < count <= N
     for (int t = gtid; t < p.T; t += gsize) {
         int slot = -1;
         if (t < ntok) {
             const int r = last_le(s_tok, p.R, t);
-            const int have = min(max(p.lens[r], 0), cap);
-            const int place = have + (t - s_tok[r]), at = place >> p.shift, hp = (have + round) >> p.shift;
+            const int have = s_have[r], place = have + (t - s_tok[r]), at = place >> p.shift, hp = (have + round) >> p.shift;
             const int id = at < hp ? p.tables[(long)r * p.table_stride + at] : taken(s_grow[r] + (at - hp));
             slot = (unsigned)id < (unsigned)N ? (id << p.shift) + (place & round) : -1;
         }
@@ -141,13 +156,13 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_pages_kernel(const PlanPara
     }
     for (int i = gtid; i < ngrow; i += gsize) {
         const int r = last_le(s_grow, p.R, i);
-        const int hp = (min(max(p.lens[r], 0), cap) + round) >> p.shift;
-        p.tables[(long)r * p.table_stride + hp + (i - s_grow[r])] = taken(i);
+        p.tables[(long)r * p.table_stride + ((s_have[r] + round) >> p.shift) + (i - s_grow[r])] = taken(i);
     }
     for (int i = gtid; i < nshrink; i += gsize) {
         const int r = last_le(s_shrink, p.R, i);
         const int wp = (min(max(p.new_lens[r], 0), cap) + round) >> p.shift;
-        p.ring[((long)head + count + i) % N] = p.tables[(long)r * p.table_stride + wp + (i - s_shrink[r])];
+        // (head + count + i < 3 N: twice around at most)
+        p.ring[wrap(wrap((unsigned)head + (unsigned)count) + (unsigned)i)] = p.tables[(long)r * p.table_stride + wp + (i - s_shrink[r])];
     }
 }
 
@@ -380,13 +395,13 @@ int iggt_plan_pages(int* tables, long table_stride, int requests, int table_widt
     if (((long)table_width << shift) >= (1L << 31) - 1024 || ((long)num_pages << shift) >= (1L << 31)) return -1;
     PlanParams p = {tables, table_stride, requests, table_width, ring, num_pages, counters, lens, new_lens, shift, starts,
                     next_lens, next_counters, slots, num_slots};
-    // every workgroup repeats the prefix sums (microseconds), so only as many as the slots keep busy
-    int blocks = (num_slots + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS);
-    blocks = blocks < 1 ? 1 : (blocks > 64 ? 64 : blocks);
-    const size_t lds = (size_t)(requests > 0 ? requests : 1) * 3 * sizeof(int);
+    // every workgroup repeats the prefix sums, and then a slot per thread is the shortest
+    int blocks = (num_slots + PLAN_THREADS - 1) / PLAN_THREADS;
+    blocks = blocks < 1 ? 1 : (blocks > 256 ? 256 : blocks);
+    const size_t lds = (size_t)(requests > 0 ? requests : 1) * 4 * sizeof(int);
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void*)plan_pages_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 PLAN_MAX_REQUESTS * 3 * (int)sizeof(int));
+                                                 PLAN_MAX_REQUESTS * 4 * (int)sizeof(int));
         if (e != hipSuccess) return (int)e;
     }
     hipLaunchKernelGGL(plan_pages_kernel, dim3(blocks), dim3(PLAN_THREADS), lds, (hipStream_t)stream, p);
