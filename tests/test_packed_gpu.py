@@ -470,3 +470,110 @@ def test_calls_repeat_bit_for_bit_and_follow_the_current_stream():
         late = packed_attention(q * 1.0, k, v, cu, cu, 600, 600)
     side.synchronize()
     assert torch.equal(first, late) and torch.equal(first, packed_attention(q, k, v, cu, cu, 600, 600))
+
+
+# ------------------------------------------------------------------------------------------------ far ends of the ranges
+def test_packed_attention_offsets_beyond_32_bits():
+    """Keys whose rows lie 32 MB apart: element and byte offsets pass 2^31 and 2^32 (and a stride that a tile could not span is refused)."""
+    rows, stride = 200, 2 ** 24 - 8
+    buf = torch.zeros(rows * stride + 64, dtype=torch.float16, device="cuda")
+    k = buf.as_strided((rows, 1, 64), (stride, 64, 1))
+    v = buf.as_strided((rows, 1, 64), (stride, 64, 1), 64)
+    k.copy_(rand((rows, 1, 64), 1, torch.float16)), v.copy_(rand((rows, 1, 64), 2, torch.float16))
+    q = rand((50, 2, 64), 3, torch.float16)
+    o = packed_attention(q, k, v, R.starts([10, 40], "cuda"), R.starts([7, 193], "cuda"), 40, 193)
+    R.close(o, *R.attention(q, k, v, [10, 40], [7, 193], True))
+    with pytest.raises(_C.HipExtensionError):
+        wide = buf.as_strided((100, 1, 64), (2 ** 24, 64, 1))
+        packed_attention(q, wide, wide, R.starts([50], "cuda"), R.starts([100], "cuda"), 50, 100)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_cache_beyond_4_gib(rows):
+    """A pool of 4.6 GB of codes: the pages in use are its first and its last ones."""
+    total, heads, page, dim = 70000, 16, 64, 64
+    pages = Pages.empty(total, heads, dim, page)
+    assert pages.k_codes.numel() > 2 ** 32
+    ids = [69999, 0, 35001, 69998]
+    tables = ints([ids])
+    kv = rand((230, 2, heads, dim), 1, torch.float16)
+    slots = ints([ids[i // page] * page + i % page for i in range(230)])
+    append_pages(pages, kv[:, 0], kv[:, 1], slots)
+    q = rand((rows, heads, dim), 2, torch.float16)
+    o = paged_attention(q, pages, tables, ints([230]), rows, 230, cu_q=R.starts([rows], "cuda"))
+    few = Pages(*(t[ids].contiguous() for t in pages))
+    k, v = R.held(few, ints([[0, 1, 2, 3]]), [230])
+    R.close(o, *R.attention(q, k, v, [rows], [230], True))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [40, 130])
+def test_packed_attention_many_sequences(n, causal):
+    """Sequences of 0 to 96 tokens, ranked by length on the GPU (up to 64 of them) or not."""
+    lens = [(37 * i) % 97 for i in range(n)]
+    run_packed(lens, [max(0, x - 3) if i % 3 else x + 20 for i, x in enumerate(lens)], 3, 3, 64, "bf16", causal, seed=n)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_paged_attention_strided_rows_and_tables(dt):
+    """Queries inside a fused matrix, output inside a wider one, tables inside a larger array."""
+    lens = [90, 200, 33]
+    pages, tables = make_cache(lens, 32, 2, 128, 4)
+    wide = torch.full((3, 64), -9, dtype=torch.int32, device="cuda")
+    wide[:, 5:5 + tables.shape[1]] = tables
+    fused = rand((3, 3, 4, 128), 5, R.H16[dt])
+    out = torch.full((3, 4, 256), 7.0, dtype=R.H16[dt], device="cuda")
+    o = paged_attention(fused[:, 1], pages, wide[:, 5:5 + tables.shape[1]], ints(lens), 1, 200, out=out[:, :, 128:])
+    k, v = R.held(pages, tables, lens)
+    R.close(o, *R.attention(fused[:, 1], k, v, [1, 1, 1], lens, True))
+    assert (out[:, :, :128] == 7).all()
+
+
+def test_paged_attention_lengths_beyond_max_len():
+    """max_len only chooses the key ranges: a request that holds more is still attended to whole."""
+    lens = [9000, 20]
+    pages, tables = make_cache(lens, 64, 1, 64, 6)
+    q = rand((2, 2, 64), 7, torch.bfloat16)
+    k, v = R.held(pages, tables, lens)
+    ref, tol = R.attention(q, k, v, [1, 1], lens, True)
+    for bound in (9000, 5000, 100, 1):
+        R.close(paged_attention(q, pages, tables, ints(lens), 1, bound), ref, tol)
+
+
+def test_plan_pages_of_8192_requests():
+    import random
+
+    rng = random.Random(1)
+    n, page, width = 8192, 16, 3
+    lens = [rng.randint(0, 48) for _ in range(n)]
+    new = [rng.randint(0, 48) for _ in range(n)]
+    held = [-(-x // page) for x in lens]
+    size = sum(held) + n * 3
+    ids = list(range(size))
+    rng.shuffle(ids)
+    tables, at = [], 0
+    for h in held:
+        tables.append(ids[at:at + h] + [-1] * (width - h))
+        at += h
+    ring = [-1] * size
+    head = size - 5
+    for i, x in enumerate(ids[at:]):
+        ring[(head + i) % size] = x
+    check_plan(ints(tables), ints(ring), ints([head, size - at]), ints(lens), new, page, n * 48)
+
+
+def test_cached_values_at_the_edges_of_the_types():
+    """fp16: values up to 65 504 (their e4m3 neighbour is 65 536) and down to the subnormals; bf16: 1e30 and 1e-30 in one cache."""
+    for dt, sizes in (("f16", (65504.0, 1.0, 3e-5)), ("bf16", (1e30, 1.0, 1e-30))):
+        pages = Pages.empty(3, 1, 64, 64)
+        k, v = rand((192, 1, 64), 1, R.H16[dt]), rand((192, 1, 64), 2, torch.float32).clamp(-1, 1)
+        scale = torch.tensor(sizes, device="cuda").repeat_interleave(64)[:, None, None]
+        v = (v * scale).to(R.H16[dt])
+        append_pages(pages, k, v, torch.arange(192, dtype=torch.int32, device="cuda"))
+        q = rand((20, 1, 64), 3, R.H16[dt])
+        for n in (64, 128, 192):     # (the last keys alone decide where large values would hide the small ones)
+            tables = ints([[2, 1, 0][:n // 64]])
+            kk, vv = R.held(pages, tables, [n])
+            for rows in (1, 20):
+                o = paged_attention(q[:rows], pages, tables, ints([n]), rows, n, cu_q=R.starts([rows], "cuda"), causal=False)
+                R.close(o, *R.attention(q[:rows], kk, vv, [rows], [n], False))
