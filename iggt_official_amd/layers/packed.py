@@ -22,53 +22,41 @@ import torch
 
 from .. import _C
 
-_INT = torch.int32
+_INT, _BYTE = torch.int32, torch.uint8
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 MAX_REQUESTS = 8192
 
 
-# The checks run on every call of a few microseconds: conditions first, messages only where one fails.
+# Calls of a few microseconds: conditions first, messages only where one fails, and no object that a plain number can stand for.
+_current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _refuse(what):
     raise _C.HipExtensionError(what)
 
 
-def _call(name, device, *args):
-    """C entry on the current stream of `device`, whichever device is current."""
-    index = device.index
-    fn = getattr(_C.load(), name)
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _C._check(rc, name)
-
-
 def _strides(name, t, step):
-    """(row, head) strides of a [rows, heads, channels] operand; dimensions of one entry have none."""
+    """(address, row stride, head stride) of a [rows, heads, channels] operand; dimensions of one entry have no stride."""
     rs, hs, cs = t.stride()
-    if t.shape[0] <= 1:
-        rs = 0
-    if t.shape[1] == 1:
-        hs = 0
-    if cs != 1 or rs % step or hs % step or t.data_ptr() % (2 * step):
-        _refuse(f"{name}: channels have to be contiguous, strides multiples of {step} elements and the start aligned to {2 * step} bytes")
-    return rs, hs
+    at = t.data_ptr()
+    if cs != 1 or (rs | hs) % step or at % (2 * step):
+        rows, heads, _ = t.shape
+        rs, hs = (0 if rows <= 1 else rs), (0 if heads == 1 else hs)
+        if cs != 1 or (rs | hs) % step or at % (2 * step):
+            _refuse(f"{name}: channels have to be contiguous, strides multiples of {step} elements and the start aligned to {2 * step} bytes")
+    return at, rs, hs
 
 
 def _query(q, out, grad):
     """Checks of the query rows and of the output that hold for both attentions; returns the output."""
-    if not q.is_cuda:
-        _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
     if q.dim() != 3 or q.dtype not in _C.H16 or q.shape[2] not in HEAD_DIMS:
         _refuse(f"q: bf16 or fp16 [rows, heads, 64 | 128] expected, got {q.dtype} {tuple(q.shape)}")
     if grad and torch.is_grad_enabled():
         _refuse("packed / paged attention is forward only: an input requires gradients")
     if out is None:
         return torch.zeros_like(q, memory_format=torch.contiguous_format)
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+    if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device():
         _refuse("out has to have q's shape, type and device")
     rs, hs, _ = out.stride()
     if (rs == 0 and q.shape[0] > 1) or (hs == 0 and q.shape[1] > 1):
@@ -76,9 +64,11 @@ def _query(q, out, grad):
     return out
 
 
-def _index(name, t, n, device):
-    if t.dtype != _INT or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
-        _refuse(f"{name}: contiguous int32 [{n}] on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+def _index(name, t, n, where):
+    """Address of a contiguous int32 [n] on device number `where`."""
+    if t.dtype != _INT or t.shape != (n,) or t.get_device() != where or not t.is_contiguous():
+        _refuse(f"{name}: contiguous int32 [{n}] on cuda:{where} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _scale(scale, dim):
@@ -103,32 +93,38 @@ def packed_attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, *, causal: boo
 
     max_q, max_k: the longest sequences' lengths or more (rows of a sequence past max_q are not computed).  out: rows that belong to
     no sequence are left as they are; without it they are 0."""
+    where = q.get_device()
+    if where < 0:
+        _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
+    if where != _current():
+        with torch.cuda.device(where):
+            return packed_attention(q, k, v, cu_q, cu_k, max_q, max_k, causal=causal, scale=scale, out=out)
     out = _query(q, out, q.requires_grad or k.requires_grad or v.requires_grad)
-    device, dtype = q.device, q.dtype
+    dtype, kv = q.dtype, k.shape
     tq, hq, dim = q.shape
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != dtype or v.dtype != dtype or k.shape[2] != dim or k.device != device or v.device != device:
-        _refuse(f"k, v: {dtype} [keys, heads, {dim}] on {device} expected, got {k.dtype} {tuple(k.shape)} on {k.device} and {v.dtype} {tuple(v.shape)} on {v.device}")
-    tk, hkv, _ = k.shape
+    if len(kv) != 3 or kv != v.shape or kv[2] != dim or k.dtype != dtype or v.dtype != dtype or k.get_device() != where or v.get_device() != where:
+        _refuse(f"k, v: {dtype} [keys, heads, {dim}] on {q.device} expected, got {k.dtype} {tuple(kv)} on {k.device} and {v.dtype} {tuple(v.shape)} on {v.device}")
+    tk, hkv, _ = kv
     if hkv == 0 or hq == 0 or hq % hkv:
         _refuse(f"{hq} query heads are no multiple of {hkv} key heads")
     batch = cu_q.numel() - 1
     if batch < 0:
         _refuse("cu_q: one entry more than there are sequences expected")
-    _index("cu_q", cu_q, batch + 1, device)
-    _index("cu_k", cu_k, batch + 1, device)
+    starts = _index("cu_q", cu_q, batch + 1, where), _index("cu_k", cu_k, batch + 1, where)
     max_q, max_k = min(int(max_q), tq), min(int(max_k), tk)
     if max_q < 0 or max_k < 0:
         _refuse("max_q and max_k are lengths")
     scale = _scale(scale, dim)
-    strides = _strides("q", q, 8), _strides("k", k, 8), _strides("v", v, 8), _strides("out", out, 4)
+    rows = *_strides("q", q, 8), *_strides("k", k, 8), *_strides("v", v, 8), *_strides("out", out, 4)
     if batch == 0 or max_q == 0:
         return out
     n = _ws_bytes("iggt_packed_attn_ws_bytes", batch, max_q, max_k, hq, hkv, dim)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    _call("iggt_packed_attn_f16" if dtype == torch.float16 else "iggt_packed_attn_bf16", device,
-          q.data_ptr(), *strides[0], k.data_ptr(), *strides[1], v.data_ptr(), *strides[2], out.data_ptr(), *strides[3],
-          cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, max_q, max_k, hq, hkv, dim, scale, int(causal),
-          0 if ws is None else ws.data_ptr(), n)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    lib = _C.load()
+    rc = (lib.iggt_packed_attn_f16 if dtype == torch.float16 else lib.iggt_packed_attn_bf16)(
+        *rows, *starts, batch, tq, tk, max_q, max_k, hq, hkv, dim, scale, 1 if causal else 0, ws.data_ptr() if n else 0, n, _stream(where))
+    if rc:
+        _C._check(rc, "iggt_packed_attn")
     return out
 
 
@@ -149,7 +145,7 @@ class Pages(NamedTuple):
                      make(pages, kv_heads))
 
 
-def _pages(pages, device):
+def _pages(pages, where):
     """(number of pages, key heads, page size, head dim) of a checked cache."""
     k, ks, v, vs = pages
     n, heads, page, dim = k.shape if k.dim() == 4 else (0, 0, 0, 0)
@@ -158,8 +154,8 @@ def _pages(pages, device):
     if ks.shape != (n, heads) or vs.shape != (n, heads) or v.shape != (n, heads, page // 16, dim, 16):
         _refuse(f"cache buffers do not belong together: {[tuple(t.shape) for t in pages]}")
     for t in pages:
-        if t.dtype != torch.uint8 or t.device != device or not t.is_contiguous():
-            _refuse(f"cache buffers: contiguous uint8 on {device} expected, got {t.dtype} on {t.device}")
+        if t.dtype != _BYTE or t.get_device() != where or not t.is_contiguous():
+            _refuse(f"cache buffers: contiguous uint8 on cuda:{where} expected, got {t.dtype} on {t.device}")
     return n, heads, page, dim
 
 
@@ -168,19 +164,25 @@ def append_pages(pages: Pages, k, v, slots):
     not in the cache are skipped).  Rows of one page have to be one run of consecutive slots, as plan_pages gives them: a page that
     appears in two runs of one call has no defined content.  The scale of a page is the least power of two that holds its largest
     finite value, and never falls while the page is being filled; held codes are rewritten when it grows."""
-    device, dtype = k.device, k.dtype
-    if not k.is_cuda or k.dim() != 3 or dtype not in _C.H16:
-        _refuse("k: bf16 or fp16 [tokens, key heads, D] on a ROCm device expected (no CPU fallback)")
-    n, heads, page, dim = _pages(pages, device)
-    tokens = k.shape[0]
-    if k.shape != (tokens, heads, dim) or v.shape != k.shape or v.dtype != dtype or v.device != device:
-        _refuse(f"k, v: [tokens, {heads}, {dim}] of one type expected, got {tuple(k.shape)} {dtype} and {tuple(v.shape)} {v.dtype}")
+    where = k.get_device()
+    if where < 0:
+        _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
+    if where != _current():
+        with torch.cuda.device(where):
+            return append_pages(pages, k, v, slots)
+    dtype = k.dtype
+    n, heads, page, dim = _pages(pages, where)
+    if k.dim() != 3 or k.shape[1:] != (heads, dim) or dtype not in _C.H16 or v.shape != k.shape or v.dtype != dtype or v.get_device() != where:
+        _refuse(f"k, v: bf16 or fp16 [tokens, {heads}, {dim}] of one type expected, got {tuple(k.shape)} {dtype} and {tuple(v.shape)} {v.dtype}")
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _refuse("append_pages is forward only: an input requires gradients")
-    _index("slots", slots, tokens, device)
-    _call("iggt_append_pages_f16" if dtype == torch.float16 else "iggt_append_pages_bf16", device,
-          k.data_ptr(), *_strides("k", k, 8), v.data_ptr(), *_strides("v", v, 8), slots.data_ptr(), tokens,
-          pages.k_codes.data_ptr(), pages.k_scale.data_ptr(), pages.v_codes.data_ptr(), pages.v_scale.data_ptr(), n, page, heads, dim)
+    tokens = k.shape[0]
+    lib = _C.load()
+    rc = (lib.iggt_append_pages_f16 if dtype == torch.float16 else lib.iggt_append_pages_bf16)(
+        *_strides("k", k, 8), *_strides("v", v, 8), _index("slots", slots, tokens, where), tokens, pages.k_codes.data_ptr(),
+        pages.k_scale.data_ptr(), pages.v_codes.data_ptr(), pages.v_scale.data_ptr(), n, page, heads, dim, _stream(where))
+    if rc:
+        _C._check(rc, "iggt_append_pages")
     return pages
 
 
@@ -192,39 +194,48 @@ def paged_attention(q, pages: Pages, tables, lens, max_q: int, max_len: int, *, 
 
     max_q, max_len: the largest number of rows, of tokens, or more.  Tokens on a page that does not exist count as not there.  out:
     as in packed_attention."""
+    where = q.get_device()
+    if where < 0:
+        _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
+    if where != _current():
+        with torch.cuda.device(where):
+            return paged_attention(q, pages, tables, lens, max_q, max_len, cu_q=cu_q, causal=causal, scale=scale, out=out)
     out = _query(q, out, q.requires_grad)
-    device, dtype = q.device, q.dtype
+    dtype = q.dtype
     tq, hq, dim = q.shape
-    n, hkv, page, d = _pages(pages, device)
+    n, hkv, page, d = _pages(pages, where)
     if d != dim or hq == 0 or hq % hkv:
         _refuse(f"q has {hq} heads of {dim}, the cache {hkv} of {d}")
-    batch, width, stride = _tables(tables, device, page)
-    _index("lens", lens, batch, device)
+    batch, width, stride = _tables(tables, where, page)
+    held = _index("lens", lens, batch, where)
     max_q, max_len = min(int(max_q), tq), min(int(max_len), width * page)
     if max_q < 0 or max_len < 0:
         _refuse("max_q and max_len are lengths")
+    starts = 0
     if cu_q is not None:
-        _index("cu_q", cu_q, batch + 1, device)
+        starts = _index("cu_q", cu_q, batch + 1, where)
     elif max_q > 1 or tq < batch:
         _refuse("without cu_q there is one row per request")
     scale = _scale(scale, dim)
-    strides = _strides("q", q, 8), _strides("out", out, 4)
+    rows = *_strides("q", q, 8), *_strides("out", out, 4)
     if batch == 0 or max_q == 0:
         return out
     nbytes = _ws_bytes("iggt_paged_attn_ws_bytes", batch, max_q, max_len, hq, hkv, dim)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _call("iggt_paged_attn_f16" if dtype == torch.float16 else "iggt_paged_attn_bf16", device,
-          q.data_ptr(), *strides[0], out.data_ptr(), *strides[1],
-          pages.k_codes.data_ptr(), pages.k_scale.data_ptr(), pages.v_codes.data_ptr(), pages.v_scale.data_ptr(), n, page,
-          tables.data_ptr(), stride, width, lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), batch, tq, max_q,
-          max_len, hq, hkv, dim, scale, int(causal), 0 if ws is None else ws.data_ptr(), nbytes)
+    ws = torch.empty(nbytes, dtype=_BYTE, device=q.device) if nbytes else None
+    lib = _C.load()
+    rc = (lib.iggt_paged_attn_f16 if dtype == torch.float16 else lib.iggt_paged_attn_bf16)(
+        *rows, pages.k_codes.data_ptr(), pages.k_scale.data_ptr(), pages.v_codes.data_ptr(), pages.v_scale.data_ptr(), n, page,
+        tables.data_ptr(), stride, width, held, starts, batch, tq, max_q, max_len, hq, hkv, dim, scale, 1 if causal else 0,
+        ws.data_ptr() if nbytes else 0, nbytes, _stream(where))
+    if rc:
+        _C._check(rc, "iggt_paged_attn")
     return out
 
 
-def _tables(tables, device, page):
+def _tables(tables, where, page):
     """(requests, width, row stride) of checked block tables."""
-    if tables.dim() != 2 or tables.dtype != _INT or tables.device != device:
-        _refuse(f"tables: int32 [requests, pages of the longest] on {device} expected, got {tables.dtype} {tuple(tables.shape)} on {tables.device}")
+    if tables.dim() != 2 or tables.dtype != _INT or tables.get_device() != where:
+        _refuse(f"tables: int32 [requests, pages of the longest] on cuda:{where} expected, got {tables.dtype} {tuple(tables.shape)} on {tables.device}")
     requests, width = tables.shape
     rs, cs = tables.stride()
     if (width > 1 and cs != 1) or (requests > 1 and rs < width):
@@ -243,27 +254,30 @@ def plan_pages(tables, ring, counters, lens, new_lens, page: int, tokens: int):
     Returns (tables, ring, starts [R + 1], next_lens [R], next_counters [3] = (head, count, missing), slots [tokens]): slots of the
     added tokens in request order, -1 behind the last, request b's at starts[b] .. starts[b + 1].  `missing` pages > 0 (or -1: `tokens` is
     too small) means that no request has grown in this step."""
-    device = tables.device
-    if not tables.is_cuda:
+    where = tables.get_device()
+    if where < 0:
         _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
+    if where != _current():
+        with torch.cuda.device(where):
+            return plan_pages(tables, ring, counters, lens, new_lens, page, tokens)
     if page not in PAGE_SIZES:
         _refuse(f"pages hold {PAGE_SIZES} tokens, not {page}")
-    requests, width, stride = _tables(tables, device, page)
+    requests, width, stride = _tables(tables, where, page)
     tokens, size = int(tokens), ring.numel()
     if requests > MAX_REQUESTS or tokens < 0 or size * page >= 2 ** 31:
         _refuse(f"at most {MAX_REQUESTS} requests and 2^31 slots")
-    _index("ring", ring, size, device)
     if counters.numel() < 2:
         _refuse("counters: int32 (head, count, ...) expected")
-    _index("counters", counters, counters.numel(), device)
-    _index("lens", lens, requests, device)
-    _index("new_lens", new_lens, requests, device)
-    buf = torch.empty(2 * requests + 4 + tokens, dtype=_INT, device=device)     # one allocation for the four outputs
+    inputs = (_index("counters", counters, counters.numel(), where), _index("lens", lens, requests, where),
+              _index("new_lens", new_lens, requests, where))
+    free = _index("ring", ring, size, where)
+    buf = torch.empty(2 * requests + 4 + tokens, dtype=_INT, device=tables.device)     # one allocation for the four outputs
     starts, next_lens, next_counters, slots = buf.split((requests + 1, requests, 3, tokens))
-    base = buf.data_ptr()
-    _call("iggt_plan_pages", device, tables.data_ptr(), stride, requests, width, ring.data_ptr(), size,
-          counters.data_ptr(), lens.data_ptr(), new_lens.data_ptr(), page, base, base + 4 * (requests + 1), base + 4 * (2 * requests + 1),
-          base + 4 * (2 * requests + 4), tokens)
+    at = buf.data_ptr()
+    rc = _C.load().iggt_plan_pages(tables.data_ptr(), stride, requests, width, free, size, *inputs, page, at, at + 4 * (requests + 1),
+                                   at + 4 * (2 * requests + 1), at + 4 * (2 * requests + 4), tokens, _stream(where))
+    if rc:
+        _C._check(rc, "iggt_plan_pages")
     return tables, ring, starts, next_lens, next_counters, slots
 
 
