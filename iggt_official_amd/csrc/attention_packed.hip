@@ -73,9 +73,10 @@ IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt
     }
 }
 
-template <int D, int QB, int KVM, int FMT, bool PAGED>
-__global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnParams p) {
-    constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, TILE = 2 * K_BYTES, BUF = KVM * TILE, NKC = D / 16, NDH = D / 32, BM = 128 * QB;
+template <int D, int QB, int NW, int KVM, int FMT, bool PAGED>
+__global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttnParams p) {
+    constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, TILE = 2 * K_BYTES, BUF = KVM * TILE, NKC = D / 16, NDH = D / 32, BM = 32 * NW * QB;
+    constexpr int NT = 64 * NW;   // threads
     constexpr int SLOTS = ROWB / 16;   // 16-byte slots of a K row
     __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     // ---- staging.  16-bit: LDS-DMA, 1 KiB per wave and instruction; the row-image swizzles are applied to the source piece, rows
     //      past the end are clamped to the last key (masked; see the file comment for values that are not finite).
     constexpr int RPC = 1024 / ROWB;            // rows of a 1 KiB chunk
-    constexpr int CPW = K_BYTES / 1024 / 4;     // chunks per wave
+    constexpr int CPW = K_BYTES / 1024 / NW;    // chunks per wave
     const bf16_t* kb_ptr = nullptr;
     const bf16_t* vb_ptr = nullptr;
     // the lane's piece of chunk i is in row wave CPW RPC + i RPC + lane / SLOTS of the tile, at the swizzled byte column kcol ^ flip(i) of
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     const int drow = wave * (CPW * RPC) + lane / SLOTS, pos = lane % SLOTS;
     const int kcol = (D == 64 ? pos ^ ((drow >> 1) & 7) : pos ^ (drow & 15)) * 16;
     const int vcol = (D == 64 ? (((pos >> 1) ^ (drow & 2)) << 1) | (pos & 1) : (((pos >> 1) ^ ((drow & 3) << 1)) << 1) | (pos & 1)) * 16;
-    static_assert(RPC * CPW == 16, "a wave's rows begin at a multiple of 16");
+    static_assert(CPW <= 1 || (RPC * CPW) % 8 == 0, "a wave's rows begin where the swizzle does");
     uint32_t koff0 = 0, voff0 = 0;              // byte offset of the first chunk's piece (host: a tile spans less than 2^32)
     if constexpr (!PAGED) {
         kb_ptr = p.k + (long)sp.k0 * p.k_rs + (long)h * p.k_hs;
@@ -160,21 +161,26 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     // [D][64 keys] with the keys of every 16 in the order 0-3, 8-11 | 4-7, 12-15 (what the two lane halves need side by side).
     // fp16 holds half of each value (a code of a scale near fp16's range would round to 2^16): the factor 2 of K goes into the softmax
     // scale, that of V into the epilogue.
-    constexpr int PPT = D / 64;   // 16-byte pieces of K (and of V) per thread
+    constexpr int PIECES = 4 * D;                                       // 16-byte pieces of K in a tile, and of V
+    constexpr int PPT = PIECES > NT ? PIECES / NT : 1;                  // a thread's of each
+    constexpr bool APART = PIECES < NT;                                 // the first half of the waves takes K, the second V
     constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
     u32x4 k8r[PPT], v8r[PPT];
     uint32_t kbyte[PPT], vbyte[PPT];
     uint32_t have = 0xf, have1 = 0xf, have2 = 0xf;   // which 16-key groups have a page: this tile, the next one, the one after it
-    // a wave's piece i lies in one 16-key group: one table entry (lane l: group l & 3), loaded a tile ahead, serves its K and, a tile
-    // later, its V
-    const int psub = D == 64 ? wave : wave >> 1, pin16 = D == 64 ? lane : (wave & 1) * 64 + lane;   // group of piece i less 2 i; piece of the group
+    // a wave's piece i lies in one 16-key group of D pieces: one table entry (lane l: group l & 3), loaded a tile ahead, serves its K
+    // and, a tile later, its V
+    const int first_piece = APART ? tid & (PIECES - 1) : tid;
+    const int psub = __builtin_amdgcn_readfirstlane(first_piece / D), pin16 = first_piece % D;   // group (+ i NT / D) and piece within it
+    const bool takes_k = !APART || wave < NW / 2, takes_v = !APART || wave >= NW / 2;
     int pid_v = 0, pid_k = 0;
     auto look_up = [&](int t) { return page_entry(p, b, t * 64 + (lane & 3) * 16); };
     auto groups = [&](int pid) { return (uint32_t)__ballot(page_ok(p, pid)) & 0xfu; };
     auto fetch = [&](bool V, int t, int pid, u32x4 (&code)[PPT], uint32_t (&byte)[PPT]) {
+        if (V ? !takes_v : !takes_k) return;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
-            const int sub = psub + 2 * i, id = __builtin_amdgcn_readlane(pid, sub);
+            const int sub = psub + i * (NT / D), id = __builtin_amdgcn_readlane(pid, sub);
             const long head = (long)(page_ok(p, id) ? id : 0) * p.Hkv + h;
             const long at = ((head << p.page_shift) + ((t * 64 + sub * 16) & ((1 << p.page_shift) - 1))) * D + pin16 * 16;
             byte[i] = (V ? p.v_scale : p.k_scale)[head];
@@ -182,9 +188,10 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         }
     };
     auto stage_k = [&](char* sK) {
+        if (!takes_k) return;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
-            const int key = (psub + 2 * i) * 16 + pin16 / (D / 16), piece = pin16 % (D / 16), sw = D == 64 ? (key >> 1) & 7 : key & 15;
+            const int key = (psub + i * (NT / D)) * 16 + pin16 / (D / 16), piece = pin16 % (D / 16), sw = D == 64 ? (key >> 1) & 7 : key & 15;
             bf16x8 lo, hi;
             cvt16<FMT>(k8r[i], scale_of(kbyte[i]) * HALF, lo, hi);
             *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece) ^ sw) * 16) = lo;
@@ -192,9 +199,10 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
         }
     };
     auto stage_v = [&](char* sV) {
+        if (!takes_v) return;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
-            const int sub = psub + 2 * i;
+            const int sub = psub + i * (NT / D);
             bf16x8 lo, hi;
             cvt16<FMT>(v8r[i], scale_of(vbyte[i]) * HALF, lo, hi);
             const u32x4 a = __builtin_bit_cast(u32x4, lo), z = __builtin_bit_cast(u32x4, hi);
@@ -386,7 +394,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
             }
         }
         __syncthreads();
-        for (int i = tid * 4; i < K_BYTES; i += 1024) {
+        for (int i = tid * 4; i < K_BYTES; i += 4 * NT) {
             uint32_t w = *reinterpret_cast<const uint32_t*>(sV + i);
             if (nonfinite2<FMT>(w & 0xffffu)) w &= 0xffff0000u;
             if (nonfinite2<FMT>(w & 0xffff0000u)) w &= 0xffffu;
@@ -407,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
 
     auto tile_nonfinite = [&](const char* sV) __attribute__((always_inline)) {
         bool bad = false;
-        for (int i = tid * 16; i < K_BYTES; i += 4096) bad = bad || nonfinite8<FMT>(*reinterpret_cast<const bf16x8*>(sV + i));
+        for (int i = tid * 16; i < K_BYTES; i += 16 * NT) bad = bad || nonfinite8<FMT>(*reinterpret_cast<const bf16x8*>(sV + i));
         return __syncthreads_or(bad) != 0;
     };
 
@@ -587,22 +595,23 @@ __global__ __launch_bounds__(256, 2) void seq_attn_tile_kernel(const SeqAttnPara
     }
 }
 
-template <int D, int QB, int KVM, int FMT, bool PAGED>
+template <int D, int QB, int NW, int KVM, int FMT, bool PAGED>
 int launch(const SeqAttnParams& p_in, hipStream_t stream) {
     SeqAttnParams p = p_in;
-    p.qtiles = (int)(((long)p.max_q * p.G + 128 * QB - 1) / (128 * QB));
+    constexpr int BM = 32 * NW * QB;
+    p.qtiles = (int)(((long)p.max_q * p.G + BM - 1) / BM);
     const long n = (long)p.qtiles * p.splits * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
-    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, KVM, FMT, PAGED>), dim3((unsigned)n), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, KVM, FMT, PAGED>), dim3((unsigned)n), dim3(64 * NW), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
 }
 
 template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
-    if (D == 128) return launch<128, 1, 1, FMT, PAGED>(p, stream);
-    if constexpr (PAGED) return launch<64, 1, 1, FMT, PAGED>(p, stream);
-    else return small ? launch<64, 1, 1, FMT, PAGED>(p, stream) : launch<64, 2, 2, FMT, PAGED>(p, stream);
+    if (small) return D == 64 ? launch<64, 1, 4, 1, FMT, PAGED>(p, stream) : launch<128, 1, 4, 1, FMT, PAGED>(p, stream);
+    if constexpr (PAGED) return launch<128, 1, 8, 1, FMT, PAGED>(p, stream);
+    else return launch<64, 2, 4, 2, FMT, PAGED>(p, stream);
 }
 
 }  // namespace
@@ -612,22 +621,30 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
     return paged ? launch_fmt<FMT_BF16, true>(p, D, small, stream) : launch_fmt<FMT_BF16, false>(p, D, small, stream);
 }
 
-// Key ranges of a grid of `items` tiles that does not fill the chip.  The fullest CU has n = ceil(items s / 256) work items, each 1 / s of
-// a tile's keys; it runs them two at a time, and one alone at about 0.55 of the rate.  The fold moves 8 D bytes per row and range,
-// 240 s / keys of the tiles' own time at the rates of this card.
+// Tile height and key ranges.  128-row tiles (four waves), but
+//   16-bit keys, head dim 64: 256 rows (two query blocks per wave) where they fill the chip twice;
+//   8-bit keys, head dim 128: 256 rows (eight waves) for more than 128 rows -- the workgroup converts the keys it reads, and half of that
+//   work per row is worth the coupling of eight waves (1 374 rows against 10 175 tokens, 5 x 8 heads: 540 -> 420 us; with head dim 64
+//   it is not: 256 -> 279, nor with 16-bit keys: 974 -> 1 033).
+// Ranges, where the grid is small: the work of all items over the CUs (two run together on one, a CU with a single item has 0.55 of
+// the rate), half of an item for the tail, and the fold (a launch of 3 us; 4 D bytes per row and range written and read), in
+// microseconds at the rates measured here (a CU does 3.1 MFLOP in one, 2.2 from 8-bit keys; causal masks, unknown here, count for 0.7).
 SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D, bool paged) {
     SeqPlan plan = {};
     const long rows = max_q * G, pairs = (long)B * Hkv, cus = 256;
-    plan.small = D == 64 && (paged || rows <= 128 || pairs * ((rows + 255) / 256) < 2 * cus);
-    const int bm = (D == 128 || plan.small) ? 128 : 256;
+    plan.small = paged ? (D == 64 || rows <= 128) : (D == 128 || rows <= 128 || pairs * ((rows + 255) / 256) < 2 * cus);
+    const int bm = plan.small ? 128 : 256;
     const long items = pairs * ((rows + bm - 1) / bm);
     plan.splits = 1;
-    if (items < 4 * cus && max_k >= 1024) {
-        const long most = max_k / 512 < 32 ? max_k / 512 : 32;      // at least eight tiles per range
+    if (items < 4 * cus && max_k >= 512) {
+        const double item_us = 4.0 * D * bm * max_k / (paged ? 2.2e6 : 3.1e6);
+        const double fold_us = 8.0 * D * pairs * rows / 4.0e6;
+        const long most = max_k / 256 < 32 ? max_k / 256 : 32;      // at least four tiles per range
         double best = 1e30;
         for (long s = 1; s <= most; ++s) {
-            const long n = (items * s + cus - 1) / cus;
-            const double cost = ((double)(n / 2 * 2) + (n % 2) / 0.55) / s + (s > 1 ? (double)items / cus * 240.0 * s / max_k : 0.0);
+            const double n = (double)items * s / cus;
+            const double busy = n <= 1.0 ? 1.0 / 0.55 : n <= 2.0 ? 2.0 : n + 0.5;
+            const double cost = item_us * (0.7 * busy + 0.5) / s + (s > 1 ? 3.0 + fold_us * s : 0.0);
             if (cost < best * 0.97) {
                 best = cost;
                 plan.splits = (int)s;

@@ -36,19 +36,22 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int npairs = p.B * p.Hkv;
-    const int pair = blockIdx.x % npairs, split = blockIdx.x / npairs;
+    // (the 16-row tiles of one pair and key range lie npairs work items apart: with a multiple of 8 pairs on one XCD, and in any case
+    // together in time, so that the codes come from memory once)
+    const int pair = blockIdx.x % npairs, rest = blockIdx.x / npairs;
+    const int row0 = rest % p.qtiles * 16, split = rest / p.qtiles;
     const int b = pair / p.Hkv, h = pair - b * p.Hkv;
     const SeqSpan sp = seq_span<true>(p, b);
-    const int rows = sp.lq * p.G;
+    const int rows = min(sp.lq * p.G - row0, 16);
     if (rows <= 0) return;
     const int off = sp.lk - sp.lq;
     const int kend = sp.lk;
-    const int first = p.causal ? max(min(sp.lk, off + 1), 0) : sp.lk;    // keys that every row sees
+    const int first = p.causal ? max(min(sp.lk, off + row0 / p.G + 1), 0) : sp.lk;    // keys that every row sees
     // key range of the work item: whole rounds of the four waves (256 keys), of the same length for every request
     const int b0 = split * p.range_blocks;
     const int b1 = split == p.splits - 1 ? (kend + 63) >> 6 : min(b0 + p.range_blocks, (kend + 63) >> 6);   // (max_len may be too small)
 
-    const int rn = min(n, rows - 1), qi = rn / p.G, hq = h * p.G + rn - qi * p.G;
+    const int rn = row0 + min(n, rows - 1), qi = rn / p.G, hq = h * p.G + rn - qi * p.G;
     const int lim = p.causal ? max(min(sp.lk, off + qi + 1), 0) : sp.lk;
     bf16x8 qf[NC][2];
     {
@@ -239,7 +242,7 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
             ll += s_ml[w][r][1] * f;
             acc += *reinterpret_cast<const f32x4*>(&s_o[w][r][d]) * f;
         }
-        const int i = r / p.G, hr = h * p.G + r - i * p.G;
+        const int i = (row0 + r) / p.G, hr = h * p.G + row0 + r - i * p.G;
         if (p.splits > 1) {
             const long at = (((long)split * p.B + b) * p.max_q + i) * p.Hq + hr;
             if (d == 0) {
@@ -378,8 +381,10 @@ int launch_fold(const SeqAttnParams& p, hipStream_t stream) {
 }
 
 template <int D>
-int launch_rows(const SeqAttnParams& p, int fmt, hipStream_t stream) {
-    const long n = (long)p.splits * p.B * p.Hkv;
+int launch_rows(const SeqAttnParams& p_in, int fmt, hipStream_t stream) {
+    SeqAttnParams p = p_in;
+    p.qtiles = (int)(((long)p.max_q * p.G + 15) / 16);
+    const long n = (long)p.splits * p.qtiles * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
     const dim3 grid((unsigned)n), block(256);
     if (fmt == FMT_F16) {
@@ -393,17 +398,24 @@ int launch_rows(const SeqAttnParams& p, int fmt, hipStream_t stream) {
     return 0;
 }
 
-// Up to 16 rows per (request, key head): the row kernel.  Its key ranges are of one length, a multiple of 256 keys, whatever the
-// requests' own lengths, so that requests of different lengths fill the chip evenly; the range is as long as leaves about 2 500
-// work items (three to five rounds of the chip) if all requests had max_len tokens, and FOLD_MAX ranges at most.
+// Few rows per (request, key head): the row kernel, a work item for every 16 of them.  Its own work grows with the 16-row tiles, the
+// tile kernel's hardly up to 128 rows, but that one reads and converts keys at a lower rate.  Measured, rows / tile kernel, us: 16
+// requests of 4 096 tokens, 4 key heads of 128: 32 rows 36 / 47, 64 rows 26 / 55, 128 rows 49 / 64; 32 requests of 2 048, 16 key heads of
+// 64: 32 rows 42 / 41, 64 rows 79 / 53; 2 of 16 384, 16 heads of 128: 64 rows 65 / 89, 128 rows 107 / 102.
+bool few_rows(int B, long max_q, long max_len, int Hkv, int G) {
+    const long rows = max_q * G, items = (long)B * Hkv * ((rows + 15) / 16);
+    return rows <= 32 || (items <= 1024 && (rows <= 64 || (rows <= 128 && max_len <= 4096)));
+}
+// Its key ranges are of one length, a multiple of 256 keys, whatever the requests' own lengths, so that requests of different lengths
+// fill the chip evenly; the range is as long as leaves about 2 500 work items (three to five rounds of the chip) if all requests had
+// max_len tokens, and FOLD_MAX ranges at most.
 // Short requests are not split: the fold is a second launch (3.4 us, and as much again of the host's time), a wave's 64 keys are
 // 0.5 us (D = 64) or 0.9 us (128).  Measured, split / not: 1 x 16 heads of 64, 1 374 tokens 8.2 / 7.3 us, 2 048 8.1 / 8.8 (in a loop of
 // calls 12.9 / 9.5), 4 096 8.6 / 12.8; 4 heads of 128, 1 374 tokens 9.7 / 10.7 (12.8 / 10.8), 2 048 9.7 / 13.3.  Pairs that fill the chip
 // gain longer: 16 x 16 heads of 64, 4 096 tokens 25.6 / 21.6.
-bool few_rows(long max_q, int G) { return max_q * G <= 16; }
 SeqPlan paged_plan(int B, long max_q, long max_len, int Hkv, int G, int D) {
-    if (!few_rows(max_q, G)) return iggt_seq_tile_plan(B, max_q, max_len, Hkv, G, D, true);
-    const long pairs = (long)B * Hkv, blocks = (max_len + 63) / 64;
+    if (!few_rows(B, max_q, max_len, Hkv, G)) return iggt_seq_tile_plan(B, max_q, max_len, Hkv, G, D, true);
+    const long pairs = (long)B * Hkv * ((max_q * G + 15) / 16), blocks = (max_len + 63) / 64;
     long want = 2560 / pairs;
     if (want > FOLD_MAX) want = FOLD_MAX;
     if (want < 1) want = 1;
@@ -462,7 +474,7 @@ static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o,
     }
     const hipStream_t st = (hipStream_t)stream;
     int rc;
-    if (few_rows(max_q, p.G)) rc = D == 64 ? launch_rows<64>(p, fmt, st) : launch_rows<128>(p, fmt, st);
+    if (few_rows(B, max_q, max_len, Hkv, p.G)) rc = D == 64 ? launch_rows<64>(p, fmt, st) : launch_rows<128>(p, fmt, st);
     else rc = iggt_launch_seq_tiles(p, D, fmt, true, plan.small, st);
     if (rc || p.splits == 1) return rc;
     return iggt_launch_seq_fold(p, D, fmt, true, st);
