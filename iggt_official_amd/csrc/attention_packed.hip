@@ -487,7 +487,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
                 if ((t0 + 1) * 64 > w_first || (PAGED && have != 0xf)) mask(t0, 0, sa, have);
                 raise_max(0, row_max(sa));
             }
-            if (t1 - t0 > 2) __syncthreads();   // (the first step loads over the tile just read)
+            if (t1 - t0 > (PAGED ? 1 : 2)) __syncthreads();   // (the first step loads over the tile just read)
             for (int t = t0; t + 1 < t1; t += 2) {
                 step(t, sa, sb, kbuf(t + 1), vbuf(t), kbuf(t), vbuf(t + 1));
                 if (t + 2 < t1) {
