@@ -217,108 +217,135 @@ IGGT_DEVINL void write_run(const AppendParams& p, int t0, int len, int page, int
     const long head = (long)page * p.Hkv + h;
     uint8_t* scale = (V ? p.v_scale : p.k_scale) + head;
     uint8_t* dst = (V ? p.v8 : p.k8) + ((head << p.shift) * D);
-    constexpr int LPR = D / 8, RPI = 64 / LPR;   // lanes of a row (8 values each), rows of one load
+    const int old = at > 0 ? (int)*scale : 0;
+    float m = 0.f;
+
+    // Rows outside the run are read as its first or last one: the maximum is the same, and what they give is not written.  (A load under
+    // a condition of its own costs more than it saves.)
+    // rows: LPR lanes of 8 values each, U loads of RPI rows in flight
+    constexpr int LPR = D / 8, RPI = 64 / LPR, U = D == 64 ? 8 : 4;
     const int lr = lane / LPR, lc = (lane % LPR) * 8;
-    // U loads in flight at a time; K of a run that fits into them is not read again
-    constexpr int U = 4;
     u32x4 x[U];
-    auto read = [&](int from) {
+    auto read_rows = [&](int from) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int i = from + j * RPI + lr;
-            x[j] = i < len ? *reinterpret_cast<const u32x4*>(src + (long)i * rs + lc) : u32x4{0u, 0u, 0u, 0u};
+            if (from + j * RPI < len) x[j] = *reinterpret_cast<const u32x4*>(src + (long)min(from + j * RPI + lr, len - 1) * rs + lc);
         }
     };
-    const int held = at > 0 ? (int)*scale : 0;
-    float m = 0.f;
-    if (len <= RPI) {    // a token, or a few: one load
-        x[0] = lr < len ? *reinterpret_cast<const u32x4*>(src + (long)lr * rs + lc) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) m = amax2<FMT>(m, x[0][q]);
-    } else {
+    auto max_rows = [&]() {
         for (int from = 0; from < len; from += U * RPI) {
-            read(from);
+            read_rows(from);
 #pragma unroll
             for (int j = 0; j < U; ++j)
+                if (from + j * RPI < len)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) m = amax2<FMT>(m, x[j][q]);
+                    for (int q = 0; q < 4; ++q) m = amax2<FMT>(m, x[j][q]);
         }
+    };
+    // V columns: 16 tokens of a channel pair per lane, LPG lanes for a group of 16 places, NB groups of a lane at a time
+    constexpr int LPG = D / 2, GPI = 64 / LPG, NB = D == 64 ? 2 : 1;
+    const int d = (lane % LPG) * 2, g0 = at >> 4, g1 = (at + len + 15) >> 4;
+    uint32_t y[NB][16];
+    u32x4 c[NB][2];             // what a group that the run does not fill holds
+    auto out_of = [&](int g) { return dst + ((long)g * D + d) * 16; };
+    auto whole = [&](int g) { return g * 16 >= at && g * 16 + 16 <= at + len; };
+    auto read_groups = [&](int from) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (from + b * GPI >= g1) continue;
+            const int gb = from + b * GPI + lane / LPG, first = gb * 16 - at;
+            if (gb < g1 && !whole(gb)) {
+                c[b][0] = *reinterpret_cast<const u32x4*>(out_of(gb));
+                c[b][1] = *reinterpret_cast<const u32x4*>(out_of(gb) + 16);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                y[b][j] = *reinterpret_cast<const uint32_t*>(src + (long)min(max(first + j, 0), len - 1) * rs + d);
+        }
+    };
+
+    const bool at_once = V && g1 - g0 <= NB * GPI;      // V of a run that fits into a lane's registers is read once
+    if constexpr (V) {
+        if (at_once) {
+            read_groups(g0);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (g0 + b * GPI < g1)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) m = amax2<FMT>(m, y[b][j]);
+        } else {
+            max_rows();
+        }
+    } else {
+        max_rows();
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const int need = scale_byte(m), old = held, now = max(old, need);
+    const int now = max(old, scale_byte(m));
     // 2^(127 - now): the last two exponents have a subnormal reciprocal (2^-127)
     const float inv = now >= 254 ? __builtin_bit_cast(float, 0x00400000u) : pow2_byte(254 - now);
     const bool moved = at > 0 && now > old;
     // 2^(old - now); below e4m3's whole range it is as good as 0
     const float down = moved ? (now - old > 40 ? 0.f : pow2_byte(127 - (now - old))) : 1.f;
-    if constexpr (!V) {
-        if (moved)
-            for (int i = lane; i < at * (D / 16); i += 64) {
-                u32x4 w = reinterpret_cast<u32x4*>(dst)[i];
+    if (moved) {    // held codes: K rows before the run, V groups before its first (that group below)
+        const int pieces = V ? g0 * D : at * (D / 16);
+        for (int i = lane; i < pieces; i += 64) {
+            u32x4 w = reinterpret_cast<u32x4*>(dst)[i];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = scale4(w[j], down);
-                reinterpret_cast<u32x4*>(dst)[i] = w;
-            }
+            for (int j = 0; j < 4; ++j) w[j] = scale4(w[j], down);
+            reinterpret_cast<u32x4*>(dst)[i] = w;
+        }
+    }
+    if constexpr (!V) {
         for (int from = 0; from < len; from += U * RPI) {
-            if (len > U * RPI) read(from);
+            if (len > U * RPI) read_rows(from);
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 const int i = from + j * RPI + lr;
-                if (i >= len) break;
-                u32x2 c;
+                if (from + j * RPI < len && i < len) {
+                    u32x2 w;
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
-                    c[q] = code4(h2_lo<FMT>(x[j][2 * q]) * inv, h2_hi<FMT>(x[j][2 * q]) * inv, h2_lo<FMT>(x[j][2 * q + 1]) * inv, h2_hi<FMT>(x[j][2 * q + 1]) * inv);
-                *reinterpret_cast<u32x2*>(dst + (long)(at + i) * D + lc) = c;
+                    for (int q = 0; q < 2; ++q)
+                        w[q] = code4(h2_lo<FMT>(x[j][2 * q]) * inv, h2_hi<FMT>(x[j][2 * q]) * inv, h2_lo<FMT>(x[j][2 * q + 1]) * inv, h2_hi<FMT>(x[j][2 * q + 1]) * inv);
+                    *reinterpret_cast<u32x2*>(dst + (long)(at + i) * D + lc) = w;
+                }
             }
         }
     } else {
-        // 16 tokens of a channel pair per lane: D / 2 lanes per group of 16 tokens
-        constexpr int LPG = D / 2, GPI = 64 / LPG;
-        const int d = (lane % LPG) * 2;
-        const int g1 = (at + len + 15) >> 4;
-        for (int g = (moved ? 0 : at >> 4) + lane / LPG; g < g1; g += GPI) {
-            const int first = g * 16 - at;    // token of the group's first place
-            uint8_t* out = dst + ((long)g * D + d) * 16;
-            u32x4 c[2];
-            const bool whole = first >= 0 && first + 16 <= len;
-            if (!whole) {
-                c[0] = *reinterpret_cast<const u32x4*>(out);
-                c[1] = *reinterpret_cast<const u32x4*>(out + 16);
-            }
-            uint32_t y[16];
+        for (int from = g0; from < g1; from += NB * GPI) {
+            if (!at_once) read_groups(from);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int i = first + j;
-                y[j] = (i >= 0 && i < len) ? *reinterpret_cast<const uint32_t*>(src + (long)i * rs + d) : 0u;
-            }
+            for (int b = 0; b < NB; ++b) {
+                const int gb = from + b * GPI + lane / LPG, first = gb * 16 - at;
+                if (gb >= g1) continue;
+                const bool full = whole(gb);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t nw[2];
-                nw[0] = code4(h2_lo<FMT>(y[4 * q]) * inv, h2_lo<FMT>(y[4 * q + 1]) * inv, h2_lo<FMT>(y[4 * q + 2]) * inv, h2_lo<FMT>(y[4 * q + 3]) * inv);
-                nw[1] = code4(h2_hi<FMT>(y[4 * q]) * inv, h2_hi<FMT>(y[4 * q + 1]) * inv, h2_hi<FMT>(y[4 * q + 2]) * inv, h2_hi<FMT>(y[4 * q + 3]) * inv);
-                if (whole) {
-                    c[0][q] = nw[0];
-                    c[1][q] = nw[1];
-                } else {
-                    uint32_t fresh = 0, before = 0;   // bytes of the run, bytes of tokens held before it
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t nw[2];
+                    nw[0] = code4(h2_lo<FMT>(y[b][4 * q]) * inv, h2_lo<FMT>(y[b][4 * q + 1]) * inv, h2_lo<FMT>(y[b][4 * q + 2]) * inv, h2_lo<FMT>(y[b][4 * q + 3]) * inv);
+                    nw[1] = code4(h2_hi<FMT>(y[b][4 * q]) * inv, h2_hi<FMT>(y[b][4 * q + 1]) * inv, h2_hi<FMT>(y[b][4 * q + 2]) * inv, h2_hi<FMT>(y[b][4 * q + 3]) * inv);
+                    if (full) {
+                        c[b][0][q] = nw[0];
+                        c[b][1][q] = nw[1];
+                    } else {
+                        uint32_t fresh = 0, before = 0;   // bytes of the run, bytes of tokens held before it
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int i = first + 4 * q + j;
-                        if (i >= 0 && i < len) fresh |= 0xffu << (8 * j);
-                        if (i < 0) before |= 0xffu << (8 * j);
-                    }
+                        for (int j = 0; j < 4; ++j) {
+                            const int i = first + 4 * q + j;
+                            if (i >= 0 && i < len) fresh |= 0xffu << (8 * j);
+                            if (i < 0) before |= 0xffu << (8 * j);
+                        }
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        uint32_t w = c[s][q];
-                        if (moved) w = (scale4(w, down) & before) | (w & ~before);
-                        c[s][q] = (nw[s] & fresh) | (w & ~fresh);
+                        for (int s = 0; s < 2; ++s) {
+                            uint32_t w = c[b][s][q];
+                            if (moved) w = (scale4(w, down) & before) | (w & ~before);
+                            c[b][s][q] = (nw[s] & fresh) | (w & ~fresh);
+                        }
                     }
                 }
+                *reinterpret_cast<u32x4*>(out_of(gb)) = c[b][0];
+                *reinterpret_cast<u32x4*>(out_of(gb) + 16) = c[b][1];
             }
-            *reinterpret_cast<u32x4*>(out) = c[0];
-            *reinterpret_cast<u32x4*>(out + 16) = c[1];
         }
     }
     if (lane == 0 && (now != old)) *scale = (uint8_t)now;
