@@ -280,33 +280,20 @@ __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams 
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float total = 0.f;
     if (live) {
-        float m[FOLD_MAX / 64], l[FOLD_MAX / 64], top = M_INIT;
-#pragma unroll
-        for (int j = 0; j < FOLD_MAX / 64; ++j) {
-            const int s = j * 64 + lane;
-            m[j] = M_INIT;
-            l[j] = 0.f;
-            if (s < p.splits) {
-                m[j] = p.part_ml[2 * (s * step + row)];
-                l[j] = p.part_ml[2 * (s * step + row) + 1];
-            }
-            top = fmaxf(top, m[j]);
+        static_assert(FOLD_MAX == 64, "a lane for every range");
+        float m = M_INIT, l = 0.f;
+        if (lane < p.splits) {
+            m = p.part_ml[2 * (lane * step + row)];
+            l = p.part_ml[2 * (lane * step + row) + 1];
         }
+        float top = m;
 #pragma unroll
         for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-#pragma unroll
-        for (int j = 0; j < FOLD_MAX / 64; ++j) {
-            m[j] = l[j] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[j] - top);
-            total += l[j] * m[j];
-        }
-        total = wave_sum(total);
-#pragma unroll
-        for (int j = 0; j < FOLD_MAX / 64; ++j) {
-            for (int s = (wave % W) * NG; s < 64; s += NG * W) {
-                if (j * 64 + s >= p.splits) break;
-                const float f = __shfl(m[j], s + gr, 64);      // 0 behind the last range
-                if (f != 0.f) acc += *reinterpret_cast<const f32x4*>(p.part_o + ((j * 64 + s + gr) * step + row) * D + d) * f;
-            }
+        const float weight = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        total = wave_sum(l * weight);
+        for (int s = (wave % W) * NG; s < p.splits; s += NG * W) {
+            const float f = __shfl(weight, s + gr, 64);      // 0 behind the last range
+            if (f != 0.f) acc += *reinterpret_cast<const f32x4*>(p.part_o + ((s + gr) * step + row) * D + d) * f;
         }
 #pragma unroll
         for (int x = LPR; x < 64; x *= 2)
@@ -408,7 +395,8 @@ bool few_rows(int B, long max_q, long max_len, int Hkv, int G) {
 }
 // Its key ranges are of one length, a multiple of 256 keys, whatever the requests' own lengths, so that requests of different lengths
 // fill the chip evenly; the range is as long as leaves about 2 500 work items (three to five rounds of the chip) if all requests had
-// max_len tokens, and FOLD_MAX ranges at most.
+// max_len tokens, and FOLD_MAX ranges at most (with 128 instead of 64 the fold costs more than the ranges give: 1 x 8 heads of 128, 100 000
+// tokens 45 / 37 us, 4 x 2 heads, 60 000 30 / 25).
 // Short requests are not split: the fold is a second launch (3.4 us, and as much again of the host's time), a wave's 64 keys are
 // 0.5 us (D = 64) or 0.9 us (128).  Measured, split / not: 1 x 16 heads of 64, 1 374 tokens 8.2 / 7.3 us, 2 048 8.1 / 8.8 (in a loop of
 // calls 12.9 / 9.5), 4 096 8.6 / 12.8; 4 heads of 128, 1 374 tokens 9.7 / 10.7 (12.8 / 10.8), 2 048 9.7 / 13.3.  Pairs that fill the chip

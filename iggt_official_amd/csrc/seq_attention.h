@@ -39,7 +39,7 @@ struct SeqAttnParams {
 };
 
 constexpr float M_INIT = -3.0e38f;   // running maximum before the first key: finite, so that a masked score (-inf) gives 2^-inf = 0
-constexpr int FOLD_MAX = 128;        // key ranges a row is folded from at most
+constexpr int FOLD_MAX = 64;         // key ranges a row is folded from at most
 constexpr float P_SHIFT_F16 = 8.0f;  // fp16 numerators are 2^(s - m + 8): the small ones stay normal; cancels in O / l
 
 struct SeqSpan {
