@@ -12,6 +12,9 @@
 //         keeps 16 keys of a channel side by side, one 16-byte load for both steps.
 // Scores are scaled by the page's 2^e in fp32; V is converted with its scale.  The next keys' K codes are loaded while this block's
 // softmax runs.  The four waves of a workgroup take every fourth block of its key range and are joined in LDS.
+// Measured (MI355X, a large copy moves 5.2 TB/s): one row, 350 784 tokens, 16 heads of 64: 123 us, 5.8 TB/s, + 5 us fold; 64 requests of
+// up to 8 192 tokens, 16 query and 4 key heads of 128: 60 us, 4.8 TB/s, + 5 us; one request of 1 374 tokens, 16 heads of 64, not split:
+// 7.5 us, the latency of five dependent loads and six blocks per wave.
 #include "seq_attention.h"
 #include "../../include/iggt_hip.h"
 
