@@ -670,11 +670,11 @@ static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const v
                            int Tk, int max_q, int max_k, int Hq, int Hkv, int D, float scale, int causal, void* ws, long ws_len,
                            void* stream) {
     if (B < 0 || Tq < 0 || Tk < 0 || max_q < 0 || max_k < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
-    if (Tk >= 0x7fffffff - 1024) return -1;
+    if (Tk >= 0x7fffffff - 1024 || (long)Tq * Hq >= (1L << 31)) return -1;
     if ((q_rs | q_hs | k_rs | k_hs | v_rs | v_hs) % 8 || (o_rs | o_hs) % 4) return -2;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || (uintptr_t)o % 8) return -2;
     if (k_rs < 0 || v_rs < 0 || k_rs >= (1L << 24) || v_rs >= (1L << 24)) return -2;   // 64 rows in 32-bit byte offsets
-    if (!(scale > 0.f)) return -3;
+    if (!(scale > 0.f && scale <= 1e38f)) return -3;
     if (B == 0 || Tq == 0 || max_q == 0) return 0;
     SeqAttnParams p = {};
     p.q = (const bf16_t*)q; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.o = (bf16_t*)o;

@@ -440,10 +440,10 @@ static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o,
     const int shift = page_shift_of(page);
     if (B < 0 || Tq < 0 || max_q < 0 || max_len < 0 || num_pages < 0 || table_width < 0 || shift < 0) return -1;
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
-    if ((long)table_width * page >= (1L << 31) - 1024 || (cu_q == nullptr && max_q > 1)) return -1;
+    if ((long)table_width * page >= (1L << 31) - 1024 || (cu_q == nullptr && max_q > 1) || (long)Tq * Hq >= (1L << 31)) return -1;
     if ((q_rs | q_hs) % 8 || (o_rs | o_hs) % 4 || (uintptr_t)q % 16 || (uintptr_t)o % 8) return -2;
     if (((uintptr_t)k_codes | (uintptr_t)v_codes) % 16) return -2;
-    if (!(scale > 0.f)) return -3;
+    if (!(scale > 0.f && scale <= 1e38f)) return -3;
     if (B == 0 || Tq == 0 || max_q == 0) return 0;
     SeqAttnParams p = {};
     p.q = (const bf16_t*)q; p.o = (bf16_t*)o;

@@ -26,6 +26,7 @@ _INT, _BYTE = torch.int32, torch.uint8
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 MAX_REQUESTS = 8192
+MAX_ROWS = 2 ** 31 - 2 ** 20     # rows, keys, slots of a call: 32-bit numbers below the Python API
 
 
 # Calls of a few microseconds: conditions first, messages only where one fails, and no object that a plain number can stand for.
@@ -54,10 +55,14 @@ def _query(q, out, grad):
         _refuse(f"q: bf16 or fp16 [rows, heads, 64 | 128] expected, got {q.dtype} {tuple(q.shape)}")
     if grad and torch.is_grad_enabled():
         _refuse("packed / paged attention is forward only: an input requires gradients")
+    if q.shape[0] * q.shape[1] >= MAX_ROWS:
+        _refuse(f"{q.shape[0]} x {q.shape[1]} query rows and heads are more than {MAX_ROWS}")
     if out is None:
         return torch.zeros_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device():
         _refuse("out has to have q's shape, type and device")
+    if out.requires_grad and torch.is_grad_enabled():
+        _refuse("packed / paged attention is forward only: out requires gradients")
     rs, hs, _ = out.stride()
     if (rs == 0 and q.shape[0] > 1) or (hs == 0 and q.shape[1] > 1):
         _refuse("out is an expanded view")
@@ -75,8 +80,8 @@ def _scale(scale, dim):
     if scale is None:
         return dim ** -0.5
     scale = float(scale)
-    if not 0.0 < scale < float("inf"):
-        _refuse(f"softmax scale has to be positive and finite, got {scale}")
+    if not 1e-37 <= scale <= 1e37:      # (a float32 below)
+        _refuse(f"softmax scale has to be positive and between 1e-37 and 1e37, got {scale}")
     return scale
 
 
@@ -89,10 +94,11 @@ def packed_attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, *, causal: boo
                      out: Optional[torch.Tensor] = None):
     """softmax(scale q k^T) v within every sequence: rows cu_q[b] .. cu_q[b + 1] of q [Tq, Hq, D] over keys cu_k[b] .. cu_k[b + 1] of
     k, v [Tk, Hkv, D] (bf16 or fp16, D 64 | 128, Hq a multiple of Hkv; query head h reads key head h // (Hq // Hkv)).  causal: row i of
-    Lq sees keys j <= i + Lk - Lq; a row that sees none is 0.  scale: default D ** -0.5.
+    Lq sees keys j <= i + Lk - Lq; a row that sees none (or only scores of -inf) is 0.  scale: default D ** -0.5.
 
-    max_q, max_k: the longest sequences' lengths or more (rows of a sequence past max_q are not computed).  out: rows that belong to
-    no sequence are left as they are; without it they are 0."""
+    max_q, max_k: the longest sequences' lengths or more (rows of a sequence past max_q are not computed; max_k only steers how the
+    work is split).  out: rows that belong to no sequence are left as they are; without it they are 0.  It may be q itself, and must not
+    overlap q in another way, nor k or v.  Prefix sums do not decrease: a row that two sequences share has the values of either."""
     where = q.get_device()
     if where < 0:
         _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
@@ -108,8 +114,8 @@ def packed_attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, *, causal: boo
     if hkv == 0 or hq == 0 or hq % hkv:
         _refuse(f"{hq} query heads are no multiple of {hkv} key heads")
     batch = cu_q.numel() - 1
-    if batch < 0:
-        _refuse("cu_q: one entry more than there are sequences expected")
+    if not 0 <= batch < MAX_ROWS or tk >= MAX_ROWS:
+        _refuse(f"cu_q: one entry more than there are sequences expected; fewer than {MAX_ROWS} sequences and keys")
     starts = _index("cu_q", cu_q, batch + 1, where), _index("cu_k", cu_k, batch + 1, where)
     max_q, max_k = min(int(max_q), tq), min(int(max_k), tk)
     if max_q < 0 or max_k < 0:
@@ -177,6 +183,8 @@ def append_pages(pages: Pages, k, v, slots):
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _refuse("append_pages is forward only: an input requires gradients")
     tokens = k.shape[0]
+    if tokens >= MAX_ROWS:
+        _refuse(f"fewer than {MAX_ROWS} tokens expected, got {tokens}")
     lib = _C.load()
     rc = (lib.iggt_append_pages_f16 if dtype == torch.float16 else lib.iggt_append_pages_bf16)(
         *_strides("k", k, 8), *_strides("v", v, 8), _index("slots", slots, tokens, where), tokens, pages.k_codes.data_ptr(),
@@ -192,8 +200,8 @@ def paged_attention(q, pages: Pages, tables, lens, max_q: int, max_len: int, *, 
     tables[b, t // page], and it holds lens[b] of them (the new ones among them).  q [Tq, Hq, D]: rows cu_q[b] .. cu_q[b + 1] of request b
     are its last tokens; cu_q None: one row per request, row b.  causal: row i of Lq sees tokens t <= i + lens[b] - Lq.
 
-    max_q, max_len: the largest number of rows, of tokens, or more.  Tokens on a page that does not exist count as not there.  out:
-    as in packed_attention."""
+    max_q, max_len: the largest number of rows, of tokens, or more (as max_q and max_k there).  Tokens on a page that does not exist
+    count as not there.  out: as in packed_attention.  fp16 rows: cached V beyond 131 008 in magnitude (written from bf16) is infinite."""
     where = q.get_device()
     if where < 0:
         _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")
@@ -207,6 +215,8 @@ def paged_attention(q, pages: Pages, tables, lens, max_q: int, max_len: int, *, 
     if d != dim or hq == 0 or hq % hkv:
         _refuse(f"q has {hq} heads of {dim}, the cache {hkv} of {d}")
     batch, width, stride = _tables(tables, where, page)
+    if batch >= MAX_ROWS:
+        _refuse(f"fewer than {MAX_ROWS} requests expected")
     held = _index("lens", lens, batch, where)
     max_q, max_len = min(int(max_q), tq), min(int(max_len), width * page)
     if max_q < 0 or max_len < 0:
@@ -264,8 +274,8 @@ def plan_pages(tables, ring, counters, lens, new_lens, page: int, tokens: int):
         _refuse(f"pages hold {PAGE_SIZES} tokens, not {page}")
     requests, width, stride = _tables(tables, where, page)
     tokens, size = int(tokens), ring.numel()
-    if requests > MAX_REQUESTS or tokens < 0 or size * page >= 2 ** 31:
-        _refuse(f"at most {MAX_REQUESTS} requests and 2^31 slots")
+    if requests > MAX_REQUESTS or requests * width >= 2 ** 31 or not 0 <= tokens < MAX_ROWS or size * page >= 2 ** 31:
+        _refuse(f"at most {MAX_REQUESTS} requests, fewer than 2^31 table entries and slots and {MAX_ROWS} new tokens expected")
     if counters.numel() < 2:
         _refuse("counters: int32 (head, count, ...) expected")
     inputs = (_index("counters", counters, counters.numel(), where), _index("lens", lens, requests, where),

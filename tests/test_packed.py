@@ -113,3 +113,12 @@ def test_reference_planner_keeps_every_page_once():
         out = [tables[b][j] for b in range(n) for j in range(-(-lens[b] // page))]
         free = [ring[(counters[0] + i) % size] for i in range(counters[1])]
         assert sorted(out + free) == list(range(size))
+
+
+def test_sizes_beyond_32_bits_are_refused_on_the_host(lib):
+    """Counts whose products or whose next step would pass 2^31: before any launch."""
+    assert _packed(lib, B=1, Tq=1 << 21, Hq=1 << 10, Hkv=1) == -1 and _paged(lib, B=1, Tq=1 << 21, Hq=1 << 10, Hkv=1) == -1
+    assert _packed(lib, scale=3e38) == -3 and _paged(lib, scale=float("inf")) == -3
+    plan = lambda R, M, T: lib.iggt_plan_pages(16, M, R, M, 16, 4, 16, 16, 16, 16, 16, 16, 16, 16, T, 0)  # noqa: E731
+    assert plan(8192, 1 << 18, 4) == -1 and plan(1, 4, 0x7fffffff) == -1
+    assert lib.iggt_append_pages_f16(16, 64, 64, 16, 64, 64, 16, 0x7fffffff, 16, 16, 16, 16, 4, 64, 1, 64, 0) == -1

@@ -577,3 +577,39 @@ def test_cached_values_at_the_edges_of_the_types():
             for rows in (1, 20):
                 o = paged_attention(q[:rows], pages, tables, ints([n]), rows, n, cu_q=R.starts([rows], "cuda"), causal=False)
                 R.close(o, *R.attention(q[:rows], kk, vv, [rows], [n], False))
+
+
+def test_calls_of_more_than_32_bits_are_refused():
+    """Expanded operands whose row counts a 32-bit number does not hold."""
+    q, cu = rand((8, 2, 64), 1, torch.float16), R.starts([8], "cuda")
+    many = q[:1].expand(2 ** 31, 2, 64)
+    idx = torch.zeros(4, dtype=torch.int32, device="cuda")
+    pages = Pages.empty(2, 2, 64, 16)
+    for call in (lambda: packed_attention(q, many, many, cu, cu, 8, 8), lambda: packed_attention(many, q, q, cu, cu, 8, 8),
+                 lambda: packed_attention(q, q, q, cu, cu, 8, 8, scale=1e39), lambda: packed_attention(q, q, q, cu, cu, 8, 8, scale=1e-50),
+                 lambda: packed_attention(q, q, q, cu, cu, 8, 8, out=torch.zeros_like(q).requires_grad_()),
+                 lambda: append_pages(pages, many, many, idx),
+                 lambda: plan_pages(idx.view(1, 4), idx, idx, idx[:1], idx[:1], 16, 2 ** 32),
+                 lambda: plan_pages(idx.view(1, 4), idx, idx, idx[:1], idx[:1], 16, 2 ** 31 - 1)):
+        with pytest.raises(_C.HipExtensionError):
+            call()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,lens,keys", [(64, [300, 1, 40], [300, 700, 0]), (128, [300, 1, 40], [300, 700, 0]), (64, [9], [5000]), (64, [2300] * 4, [2300] * 4)])
+def test_output_in_the_place_of_the_queries(dt, dim, lens, keys):
+    """out = q (a slice of a joint projection too): bit for bit what separate memory gives, packed and from the cache."""
+    g = 2
+    x = rand((sum(lens), 8 * g, dim), 5, R.H16[dt])
+    q = x[:, g:3 * g]
+    k, v = rand((sum(keys), g, dim), 6, R.H16[dt]), rand((sum(keys), g, dim), 7, R.H16[dt])
+    cu_q, cu_k = R.starts(lens, "cuda"), R.starts(keys, "cuda")
+    want = packed_attention(q, k, v, cu_q, cu_k, max(lens), max(keys))
+    mine = x.clone()[:, g:3 * g]
+    assert packed_attention(mine, k, v, cu_q, cu_k, max(lens), max(keys), out=mine) is mine and torch.equal(mine, want)
+    pages, tables = make_cache(keys, 16, g, dim)
+    held = torch.tensor(keys, dtype=torch.int32, device="cuda")
+    want = paged_attention(q, pages, tables, held, max(lens), max(keys), cu_q=cu_q)
+    mine = x.clone()[:, g:3 * g]
+    paged_attention(mine, pages, tables, held, max(lens), max(keys), cu_q=cu_q, out=mine)
+    assert torch.equal(mine, want)
