@@ -18,8 +18,9 @@
 //   head dim 128: one query block, pipelined over the tiles.  Matrix and vector pipe 51 % each, 1.85 waves.  Prompts of 12 001 and 7 645
 //     tokens, 16 query and 4 key heads, causal, bf16: 820 us, 1 010 TFLOP/s (a large library matrix product here: 1 450).  Before the
 //     pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
-//   8-bit keys: the same with the conversion in front (13.7 vector instructions per matrix instruction at head dim 64): 1 374 rows against
-//     12 366 tokens, 2 x 16 heads of 64, fp16: 224 + 13 us, 590 TFLOP/s.
+//   8-bit keys: the same with the conversion in front, shared by 256 rows where there are as many (head dim 64: two query blocks per
+//     wave, 128: eight waves).  1 374 rows against 12 366 tokens, 2 x 16 heads of 64, fp16: 237 us with the fold (one query block: 250),
+//     590 TFLOP/s; 6 x 1 374 rows against 36 343 tokens, 8 query and 2 key heads: 524 (607).
 //   small grids: the chain of one wave's tiles, 0.8 us each; loads four tiles ahead instead of one change nothing.
 //
 // Values that are not finite: a masked score is replaced, not added to, so NaN in K costs nothing.  V does: 0 * inf = NaN in the
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
                 for (int qb = 0; qb < QB; ++qb) {
                     f32x16 s[2];
                     qk(sK, qb, s);
-                    mask(t, qb, s, 0xf);
+                    mask(t, qb, s, have);
                     raise_max(qb, row_max(s));
                 }
             }
@@ -522,7 +523,8 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
     } else {
         // Two query blocks per wave, offset against each other within the tile: the score product of the second runs beside the
         // exponentials of the first, the second product of the first beside the exponentials of the second.
-        static_assert(QB == 1 || !PAGED, "paged tiles have one query block");
+        // (8-bit keys: the next tile's codes are in registers meanwhile, and go into the other buffer at its end)
+        static_assert(!PAGED || KVM == 1, "one tile of codes at a time");
         auto load = [&](int mt, char* dst) {
 #pragma unroll
             for (int sub = 0; sub < KVM; ++sub) {
@@ -533,36 +535,60 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
             }
         };
         auto step = [&](int mt, char* here, char* dst) {
-            if (mt + 1 < t1) load(mt + 1, dst);
+            if constexpr (PAGED) {
+                const int tk = min(mt + 1, t1 - 1);
+                fetch(false, tk, pid_k, k8r, kbyte);
+                fetch(true, tk, pid_k, v8r, vbyte);
+                have1 = groups(pid_k);
+                pid_k = look_up(min(mt + 2, t1 - 1));
+            } else {
+                if (mt + 1 < t1) load(mt + 1, dst);
+            }
 #pragma unroll
             for (int sub = 0; sub < KVM; ++sub) {
                 const int t = mt * KVM + sub;
                 if (t >= ktiles) break;
                 char* sK = here + sub * TILE;
                 char* sV = sK + K_BYTES;
-                if ((t + 1) * 64 > wg_first) {
+                if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
                     if (tile_nonfinite(sV)) absorb_nonfinite(sK, sV, t);
                 }
                 if (t * 64 >= w_last) continue;
-                const bool edge = (t + 1) * 64 > w_first;
+                const bool edge = (t + 1) * 64 > w_first || (PAGED && have != 0xf);
                 f32x16 s0[2], s1[2];
                 bf16x8 pf0[2][2], pf1[2][2];
                 qk(sK, 0, s0);
-                if (edge) mask(t, 0, s0, 0xf);
+                if (edge) mask(t, 0, s0, have);
                 raise_max(0, row_max(s0));
                 qk(sK, QB - 1, s1);
                 exp_pack(0, s0, pf0);
                 pin(pf0);
-                if (edge) mask(t, QB - 1, s1, 0xf);
+                if (edge) mask(t, QB - 1, s1, have);
                 raise_max(QB - 1, row_max(s1));
                 pv(sV, 0, pf0);
                 exp_pack(QB - 1, s1, pf1);
                 pv(sV, QB - 1, pf1);
             }
+            if constexpr (PAGED) {
+                stage_k(dst);
+                stage_v(dst + K_BYTES);
+                have = have1;
+            }
             arrive();
         };
         if (t0 < t1) {
-            load(t0, smem + (t0 & 1) * BUF);
+            char* first = smem + (t0 & 1) * BUF;
+            if constexpr (PAGED) {
+                const int pid = look_up(t0);
+                pid_k = look_up(min(t0 + 1, t1 - 1));
+                have = groups(pid);
+                fetch(false, t0, pid, k8r, kbyte);
+                fetch(true, t0, pid, v8r, vbyte);
+                stage_k(first);
+                stage_v(first + K_BYTES);
+            } else {
+                load(t0, first);
+            }
             arrive();
             for (int mt = t0; mt < t1; ++mt) step(mt, smem + (mt & 1) * BUF, smem + (1 - (mt & 1)) * BUF);
         }
@@ -621,7 +647,7 @@ int launch(const SeqAttnParams& p_in, hipStream_t stream) {
 template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
     if (small) return D == 64 ? launch<64, 1, 4, 1, FMT, PAGED>(p, stream) : launch<128, 1, 4, 1, FMT, PAGED>(p, stream);
-    if constexpr (PAGED) return launch<128, 1, 8, 1, FMT, PAGED>(p, stream);
+    if constexpr (PAGED) return D == 64 ? launch<64, 2, 4, 1, FMT, PAGED>(p, stream) : launch<128, 1, 8, 1, FMT, PAGED>(p, stream);
     else return launch<64, 2, 4, 2, FMT, PAGED>(p, stream);
 }
 
@@ -634,35 +660,45 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
 
 // Tile height and key ranges.  128-row tiles (four waves), but
 //   16-bit keys, head dim 64: 256 rows (two query blocks per wave) where they fill the chip twice;
-//   8-bit keys, head dim 128: 256 rows (eight waves) for more than 128 rows -- the workgroup converts the keys it reads, and half of that
-//   work per row is worth the coupling of eight waves (1 374 rows against 10 175 tokens, 5 x 8 heads: 540 -> 420 us; with head dim 64
-//   it is not: 256 -> 279, nor with 16-bit keys: 974 -> 1 033).
+//   8-bit keys: the workgroup converts the keys it reads, half of that work per row for 256 rows.  Head dim 128 (eight waves, whose
+//   coupling costs less than that: 1 374 rows against 10 175 tokens, 5 x 8 heads: 540 -> 420 us; with 16-bit keys 974 -> 1 033): more
+//   than 128 rows.  Head dim 64 (two query blocks per wave: 1 374 rows, 6 x 8 heads, 36 343 tokens 590 -> 525 us; 2 x 16 heads, 12 366
+//   tokens 250 -> 237; but 3 x 16 heads, 1 374 tokens, causal 33 -> 47, 4 heads, 2 748 tokens 24 -> 31): where the estimate below is lower.
 // Ranges, where the grid is small: the work of all items over the CUs (two run together on one, a CU with a single item has 0.55 of
 // the rate), half of an item for the tail, and the fold (a launch of 3 us; 4 D bytes per row and range written and read), in
-// microseconds at the rates measured here (a CU does 3.1 MFLOP in one, 2.2 from 8-bit keys; causal masks, unknown here, count for 0.7).
-SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D, bool paged) {
-    SeqPlan plan = {};
-    const long rows = max_q * G, pairs = (long)B * Hkv, cus = 256;
-    plan.small = paged ? (D == 64 || rows <= 128) : (D == 128 || rows <= 128 || pairs * ((rows + 255) / 256) < 2 * cus);
-    const int bm = plan.small ? 128 : 256;
-    const long items = pairs * ((rows + bm - 1) / bm);
-    plan.splits = 1;
-    if (items < 4 * cus && max_k >= 512) {
-        const double item_us = 4.0 * D * bm * max_k / (paged ? 2.2e6 : 3.1e6);
-        const double fold_us = 8.0 * D * pairs * rows / 4.0e6;
-        const long most = max_k / 256 < 32 ? max_k / 256 : 32;      // at least four tiles per range
-        double best = 1e30;
-        for (long s = 1; s <= most; ++s) {
-            const double n = (double)items * s / cus;
-            const double busy = n <= 1.0 ? 1.0 / 0.55 : n <= 2.0 ? 2.0 : n + 0.5;
-            const double cost = item_us * (0.7 * busy + 0.5) / s + (s > 1 ? 3.0 + fold_us * s : 0.0);
-            if (cost < best * 0.97) {
-                best = cost;
-                plan.splits = (int)s;
-            }
+// microseconds at the rates measured here (a CU does `rate` flop in one; causal masks, unknown here, count for 0.7).
+static SeqPlan ranges_of(int bm, double rate, long pairs, long rows, long max_k, int D, double& us) {
+    const long items = pairs * ((rows + bm - 1) / bm), cus = 256;
+    const double item_us = 4.0 * D * bm * max_k / rate, fold_us = 8.0 * D * pairs * rows / 4.0e6;
+    auto cost = [&](long s) {
+        const double n = (double)items * s / cus;
+        const double busy = n <= 1.0 ? 1.0 / 0.55 : n <= 2.0 ? 2.0 : n + 0.5;
+        return item_us * (0.7 * busy + 0.5) / s + (s > 1 ? 3.0 + fold_us * s : 0.0);
+    };
+    SeqPlan plan = {1, bm == 128, 0};
+    us = cost(1);
+    if (items >= 4 * cus || max_k < 512) return plan;
+    const long most = max_k / 256 < 32 ? max_k / 256 : 32;      // at least four tiles per range
+    for (long s = 2; s <= most; ++s) {
+        const double c = cost(s);
+        if (c < us * 0.97) {
+            us = c;
+            plan.splits = (int)s;
         }
     }
     return plan;
+}
+SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D, bool paged) {
+    const long rows = max_q * G, pairs = (long)B * Hkv;
+    double us, us256;
+    if (!paged) {
+        const bool small = D == 128 || rows <= 128 || pairs * ((rows + 255) / 256) < 2 * 256;
+        return ranges_of(small ? 128 : 256, 3.1e6, pairs, rows, max_k, D, us);
+    }
+    const SeqPlan plan = ranges_of(128, 2.2e6, pairs, rows, max_k, D, us);
+    if (rows <= 128) return plan;
+    const SeqPlan plan256 = ranges_of(256, D == 64 ? 2.7e6 : 2.2e6, pairs, rows, max_k, D, us256);
+    return D == 128 || us256 <= us ? plan256 : plan;
 }
 
 static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v,

@@ -613,3 +613,32 @@ def test_output_in_the_place_of_the_queries(dt, dim, lens, keys):
     mine = x.clone()[:, g:3 * g]
     paged_attention(mine, pages, tables, held, max(lens), max(keys), cu_q=cu_q, out=mine)
     assert torch.equal(mine, want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,lq,page,hq,hkv", [([500, 1, 0, 63, 64, 65, 127, 128, 129, 256] + [200 + i for i in range(30)], [256, 1, 0, 63, 7, 65, 127, 130, 129, 256] + [33] * 30, 16, 16, 16),
+                                                 ([1900, 1, 1000, 64, 0, 700], [63, 1, 63, 30, 0, 20], 64, 64, 16), ([2000, 1100, 70], [400, 380, 70], 128, 16, 16)])
+def test_paged_attention_of_256_row_tiles_of_64_channels(dt, causal, lens, lq, page, hq, hkv):
+    """Two query blocks per wave over 8-bit keys: tiles that end anywhere, empty requests, key ranges, shared heads."""
+    run_paged(lens, lq, page, hq, hkv, 64, dt, causal, seed=11)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_attention_of_256_row_tiles_with_bad_pages_and_nan(dt, causal):
+    lens, lq, page = [200, 330, 500] + [16] * 37, [256, 256, 256] + [16] * 37, 32
+    pages, tables = make_cache(lens, page, 16, 64, 5)
+    tables[0, 1], tables[1, 4], tables[1, 0], tables[1, 10] = -1, 10 ** 6, -7, 2 ** 30
+    last = int(tables[0, 6])
+    pages.v_codes[last, 0, 0, 5, 6] = 0x7f                   # token 198 of request 0
+    pages.k_codes[last, 1, 7, 9] = 0xff                      # token 199
+    pages.v_codes[int(tables[2, 15]), 3, 0, 7, 1] = 0xff     # token 481 of request 2
+    q = rand((sum(lq), 16, 64), 6, R.H16[dt])
+    o = paged_attention(q, pages, tables, torch.tensor(lens, dtype=torch.int32, device="cuda"), 256, 500, cu_q=R.starts(lq, "cuda"), causal=causal)
+    seen = [torch.ones(n, dtype=torch.bool, device="cuda") for n in lens]
+    seen[0][32:64] = False
+    seen[1][:32] = seen[1][128:160] = seen[1][320:] = False
+    k, v = R.held(pages, tables, lens)
+    ref, tol = R.attention(q, k, v, lq, lens, causal, seen=seen)
+    R.close(o, ref, tol)
