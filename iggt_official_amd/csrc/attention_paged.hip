@@ -493,4 +493,31 @@ int iggt_paged_attn_f16(const void* q, long q_rs, long q_hs, void* o, long o_rs,
     return paged_attn_h16(FMT_F16, q, q_rs, q_hs, o, o_rs, o_hs, k_codes, k_scale, v_codes, v_scale, num_pages, page, tables,
                           table_stride, table_width, lens, cu_q, B, Tq, max_q, max_len, Hq, Hkv, D, scale, causal, ws, ws_len, stream);
 }
+int iggt_seq_call(const long* w) {
+    auto in = [w](int i) { return (const void*)w[i]; };
+    auto idx = [w](int i) { return (const int*)w[i]; };
+    auto out = [w](int i) { return (int*)w[i]; };
+    auto num = [w](int i) { return (int)w[i]; };
+    auto real = [w](int i) { return (float)__builtin_bit_cast(double, w[i]); };
+    switch (w[0]) {
+        case IGGT_SEQ_PACKED_ATTN_BF16:
+        case IGGT_SEQ_PACKED_ATTN_F16:
+            return (w[0] == IGGT_SEQ_PACKED_ATTN_F16 ? iggt_packed_attn_f16 : iggt_packed_attn_bf16)(
+                in(1), w[2], w[3], in(4), w[5], w[6], in(7), w[8], w[9], out(10), w[11], w[12], idx(13), idx(14), num(15), num(16), num(17),
+                num(18), num(19), num(20), num(21), num(22), real(23), num(24), out(25), w[26], out(27));
+        case IGGT_SEQ_PAGED_ATTN_BF16:
+        case IGGT_SEQ_PAGED_ATTN_F16:
+            return (w[0] == IGGT_SEQ_PAGED_ATTN_F16 ? iggt_paged_attn_f16 : iggt_paged_attn_bf16)(
+                in(1), w[2], w[3], out(4), w[5], w[6], in(7), in(8), in(9), in(10), num(11), num(12), idx(13), w[14], num(15), idx(16), idx(17),
+                num(18), num(19), num(20), num(21), num(22), num(23), num(24), real(25), num(26), out(27), w[28], out(29));
+        case IGGT_SEQ_APPEND_PAGES_BF16:
+        case IGGT_SEQ_APPEND_PAGES_F16:
+            return (w[0] == IGGT_SEQ_APPEND_PAGES_F16 ? iggt_append_pages_f16 : iggt_append_pages_bf16)(
+                in(1), w[2], w[3], in(4), w[5], w[6], idx(7), num(8), out(9), out(10), out(11), out(12), num(13), num(14), num(15), num(16), out(17));
+        case IGGT_SEQ_PLAN_PAGES:
+            return iggt_plan_pages(out(1), w[2], num(3), num(4), out(5), num(6), idx(7), idx(8), idx(9), num(10), out(11), out(12), out(13),
+                                   out(14), num(15), out(16));
+    }
+    return -1;
+}
 }

@@ -553,6 +553,16 @@ int iggt_append_pages_f16(const void* k, long k_rs, long k_hs, const void* v, lo
 int iggt_plan_pages(int* tables, long table_stride, int requests, int table_width, int* ring, int num_pages, const int* counters,
                     const int* lens, const int* new_lens, int page, int* starts, int* next_lens, int* next_counters, int* slots,
                     int num_slots, void* stream);
+/* The calls above with their arguments in memory: words[0] names the call (IGGT_SEQ_*), its arguments follow in order, 8 bytes each
+ * (integers as long, scale as double).  For bindings that convert arguments one by one: thirty of them cost more than the launch. */
+#define IGGT_SEQ_PACKED_ATTN_BF16 0
+#define IGGT_SEQ_PACKED_ATTN_F16 1
+#define IGGT_SEQ_PAGED_ATTN_BF16 2
+#define IGGT_SEQ_PAGED_ATTN_F16 3
+#define IGGT_SEQ_APPEND_PAGES_BF16 4
+#define IGGT_SEQ_APPEND_PAGES_F16 5
+#define IGGT_SEQ_PLAN_PAGES 6
+int iggt_seq_call(const long* words);
 
 #ifdef __cplusplus
 }

@@ -1,6 +1,7 @@
 """CPU checks of the packed-sequence and paged-cache operators: refusals before any launch, and the references against plain
 formulas (the kernels themselves: test_packed_gpu.py)."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -122,3 +123,25 @@ def test_sizes_beyond_32_bits_are_refused_on_the_host(lib):
     plan = lambda R, M, T: lib.iggt_plan_pages(16, M, R, M, 16, 4, 16, 16, 16, 16, 16, 16, 16, 16, T, 0)  # noqa: E731
     assert plan(8192, 1 << 18, 4) == -1 and plan(1, 4, 0x7fffffff) == -1
     assert lib.iggt_append_pages_f16(16, 64, 64, 16, 64, 64, 16, 0x7fffffff, 16, 16, 16, 16, 4, 64, 1, 64, 0) == -1
+
+
+def test_calls_with_arguments_in_memory(lib):
+    """iggt_seq_call hands every argument to the call that the first word names: the same refusals, one wrong argument at a time."""
+    good = dict(packed=(16, 64, 64, 16, 64, 64, 16, 64, 64, 16, 64, 64, 16, 16, 0, 4, 4, 4, 4, 1, 1, 64, 1.0, 1, 0, 0, 0),
+                paged=(16, 64, 64, 16, 64, 64, 16, 16, 16, 16, 4, 64, 16, 4, 4, 16, 16, 0, 4, 4, 4, 1, 1, 64, 1.0, 1, 0, 0, 0),
+                append=(16, 64, 64, 16, 64, 64, 16, 0, 16, 16, 16, 16, 4, 64, 1, 64, 0), plan=(16, 4, 8193, 4, 16, 4, 16, 16, 16, 64, 16, 16, 16, 16, 4, 0))
+    for layout, op, name, key in ((P._PACKED, 0, "iggt_packed_attn_bf16", "packed"), (P._PACKED, 1, "iggt_packed_attn_f16", "packed"),
+                                  (P._PAGED, 2, "iggt_paged_attn_bf16", "paged"), (P._PAGED, 3, "iggt_paged_attn_f16", "paged"),
+                                  (P._APPEND, 4, "iggt_append_pages_bf16", "append"), (P._APPEND, 5, "iggt_append_pages_f16", "append"),
+                                  (P._PLAN, 6, "iggt_plan_pages", "plan")):
+        args, codes = good[key], set()
+        assert struct.calcsize(layout.format) == 8 * (len(args) + 1)
+        for i in range(len(args)):
+            for wrong in (-1, 3):
+                if key == "plan" and i == 2 or key != "plan" and args[i] == 0 and i in (7, 14, 17):
+                    continue                            # these keep the call from a launch
+                a = args[:i] + (type(args[i])(wrong),) + args[i + 1:]
+                codes.add(lib.iggt_seq_call(layout.pack(op, *a)))
+                assert lib.iggt_seq_call(layout.pack(op, *a)) == getattr(lib, name)(*a), (name, i, wrong)
+        assert -1 in codes
+    assert lib.iggt_seq_call(P._PLAN.pack(7, *good["plan"])) == -1
