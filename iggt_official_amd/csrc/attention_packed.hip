@@ -19,8 +19,8 @@
 //     tokens, 16 query and 4 key heads, causal, bf16: 820 us, 1 010 TFLOP/s (a large library matrix product here: 1 450).  Before the
 //     pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
 //   8-bit keys: the same with the conversion in front, shared by 256 rows where there are as many (head dim 64: two query blocks per
-//     wave, 128: eight waves).  1 374 rows against 12 366 tokens, 2 x 16 heads of 64, fp16: 237 us with the fold (one query block: 250),
-//     590 TFLOP/s; 6 x 1 374 rows against 36 343 tokens, 8 query and 2 key heads: 524 (607).
+//     wave, 128: eight waves).  1 374 rows against 12 366 tokens, 2 x 16 heads of 64, fp16: 228 us with the fold (one query block: 250),
+//     610 TFLOP/s; 6 x 1 374 rows against 36 343 tokens, 8 query and 2 key heads: 524 (607).
 //   small grids: the chain of one wave's tiles, 0.8 us each; loads four tiles ahead instead of one change nothing.
 //
 // Values that are not finite: a masked score is replaced, not added to, so NaN in K costs nothing.  V does: 0 * inf = NaN in the
@@ -28,6 +28,7 @@
 // it holds inf or NaN they are added to exactly the rows that see them and the product runs on zeros in their place.
 #include "seq_attention.h"
 #include "../../include/iggt_hip.h"
+#include <cmath>
 
 using namespace iggt_seq;
 
@@ -665,14 +666,16 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
 //   than 128 rows.  Head dim 64 (two query blocks per wave: 1 374 rows, 6 x 8 heads, 36 343 tokens 590 -> 525 us; 2 x 16 heads, 12 366
 //   tokens 250 -> 237; but 3 x 16 heads, 1 374 tokens, causal 33 -> 47, 4 heads, 2 748 tokens 24 -> 31): where the estimate below is lower.
 // Ranges, where the grid is small: the work of all items over the CUs (two run together on one, a CU with a single item has 0.55 of
-// the rate), half of an item for the tail, and the fold (a launch of 3 us; 4 D bytes per row and range written and read), in
-// microseconds at the rates measured here (a CU does `rate` flop in one; causal masks, unknown here, count for 0.7).
+// the rate; with n per CU the last to finish has between n and ceil(n)), half of an item for the tail, and the fold (a launch of 3 us;
+// 4 D bytes per row and range written and read), in microseconds at the rates measured here (a CU does `rate` flop in one; causal
+// masks, unknown here, count for 0.7).  192 items of 256 rows, 12 366 tokens, tile kernel: 265 us in 2 ranges, 271 in 3, 233 in 4, 237 in
+// 5, 245 in 6, 235 in 8; with n + 1/2 in place of the mean of n and ceil(n) it took 6.
 static SeqPlan ranges_of(int bm, double rate, long pairs, long rows, long max_k, int D, double& us) {
     const long items = pairs * ((rows + bm - 1) / bm), cus = 256;
     const double item_us = 4.0 * D * bm * max_k / rate, fold_us = 8.0 * D * pairs * rows / 4.0e6;
     auto cost = [&](long s) {
         const double n = (double)items * s / cus;
-        const double busy = n <= 1.0 ? 1.0 / 0.55 : n <= 2.0 ? 2.0 : n + 0.5;
+        const double alone = 1.0 / 0.55, even = 0.5 * (n + std::ceil(n)) + 0.1, busy = even > alone ? even : alone;
         return item_us * (0.7 * busy + 0.5) / s + (s > 1 ? 3.0 + fold_us * s : 0.0);
     };
     SeqPlan plan = {1, bm == 128, 0};
@@ -698,7 +701,7 @@ SeqPlan iggt_seq_tile_plan(int B, long max_q, long max_k, int Hkv, int G, int D,
     const SeqPlan plan = ranges_of(128, 2.2e6, pairs, rows, max_k, D, us);
     if (rows <= 128) return plan;
     const SeqPlan plan256 = ranges_of(256, D == 64 ? 2.7e6 : 2.2e6, pairs, rows, max_k, D, us256);
-    return D == 128 || us256 <= us ? plan256 : plan;
+    return D == 128 || us256 <= 1.04 * us ? plan256 : plan;
 }
 
 static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v,
