@@ -11,13 +11,15 @@
 // Rounding: scores, maxima, sums and O are fp32; the numerators are rounded to the operand type for the second product (the row sum
 // adds them before that rounding), O once on the way out (a mean of values of that type: not saturated, inf and NaN stay).
 //
-// What bounds it (MI355X; one box, clocks fall to 1.95 GHz under this load):
-//   head dim 64, 16-bit keys: two query blocks of a wave, offset within the tile (256-row tiles).  10.8 vector instructions per matrix
-//     instruction: the vector pipe is 72 % busy, the matrix pipe 45 %, 1.8 of 2 waves per SIMD.  4 sequences of up to 10 992 tokens, 16
-//     heads, full, fp16: 1 235 us, 890 TFLOP/s.  One block per wave and four tiles in LDS: 1 403.
+// What bounds it (MI355X):
+//   head dim 64, 16-bit keys: one query block per wave, nothing overlapped within it but four waves on a SIMD (128 registers).  Vector
+//     pipe 81 % busy, matrix pipe 47 %.  4 sequences of up to 10 992 tokens, 16 heads, full, fp16: 1 207 - 1 240 us, 900 TFLOP/s, at a
+//     clock that this load pulls down to 1.7 GHz.  Two waves per SIMD with two query blocks each, offset against each other: the same
+//     there, 8 x 1 374 causal tokens 71 -> 57, 3 x 1 374 full 55 -> 48; pipelined over the tiles: 4 x 5 496 full 619 -> 590, 16 x 1 374
+//     causal 118 -> 100, but where less than two waves come to a SIMD up to 9 % faster (2 748 causal tokens 44 us, here 48).
 //   head dim 128: one query block, pipelined over the tiles.  Matrix and vector pipe 51 % each, 1.85 waves.  Prompts of 12 001 and 7 645
-//     tokens, 16 query and 4 key heads, causal, bf16: 820 us, 1 010 TFLOP/s (a large library matrix product here: 1 450).  Before the
-//     pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
+//     tokens, 16 query and 4 key heads, causal, bf16: 800 - 830 us, 1 010 TFLOP/s at 1.95 GHz (a large library matrix product here:
+//     1 450).  Before the pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
 //   8-bit keys: the same with the conversion in front, shared by 256 rows where there are as many (head dim 64: two query blocks per
 //     wave, 128: eight waves).  1 374 rows against 12 366 tokens, 2 x 16 heads of 64, fp16: 228 us with the fold (one query block: 250),
 //     610 TFLOP/s; 6 x 1 374 rows against 36 343 tokens, 8 query and 2 key heads: 524 (607).
@@ -86,12 +88,19 @@ IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt
     }
 }
 
-template <int D, int QB, int NW, int KVM, int FMT, bool PAGED>
-__global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttnParams p) {
-    constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, TILE = 2 * K_BYTES, BUF = KVM * TILE, NKC = D / 16, NDH = D / 32, BM = 32 * NW * QB;
+// Head dim 64, 16-bit keys: a wave needs 128 registers without a second tile's scores, so that four run on a SIMD and fill each other's
+// waits; the others have 256 and overlap matrix and vector work within a wave.
+constexpr int waves_per_simd(int D, int QB, bool PAGED) {
+    return D == 64 && QB == 1 && !PAGED ? 4 : 2;
+}
+
+template <int D, int QB, int NW, int FMT, bool PAGED>
+__global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_attn_tile_kernel(const SeqAttnParams p) {
+    constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, TILE = 2 * K_BYTES, NKC = D / 16, NDH = D / 32, BM = 32 * NW * QB;
+    constexpr bool PIPELINED = QB == 1 && waves_per_simd(D, QB, PAGED) == 2;   // over the tiles
     constexpr int NT = 64 * NW;   // threads
     constexpr int SLOTS = ROWB / 16;   // 16-byte slots of a K row
-    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int frow = lane & 31, fhalf = lane >> 5;
@@ -108,8 +117,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
     };
     const int kend = limit_of(min(row0 + BM, rows) - 1);
     const int ktiles = (kend + 63) >> 6;
-    const int mtiles = (ktiles + KVM - 1) / KVM;                    // macro tiles of 64 KVM keys: one barrier each
-    const int t0 = (int)((long)mtiles * split / p.splits), t1 = (int)((long)mtiles * (split + 1) / p.splits);
+    const int t0 = (int)((long)ktiles * split / p.splits), t1 = (int)((long)ktiles * (split + 1) / p.splits);
 
     const int wg_first = limit_of(row0);   // keys every row of the tile sees
     const long wrow = row0 + wave * (32 * QB);
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
     // infinities, add them to the rows that see them and leave zeros for the matrix product
     auto absorb_nonfinite = [&](char* sK, char* sV, int t) __attribute__((always_inline)) {
         if (t * 64 < w_last) {
-            if constexpr (QB == 2) {
+            if constexpr (!PIPELINED) {
 #pragma unroll
                 for (int qb = 0; qb < QB; ++qb) {
                     f32x16 s[2];
@@ -432,7 +440,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
         return __syncthreads_or(bad) != 0;
     };
 
-    if constexpr (QB == 1) {
+    if constexpr (PIPELINED) {
         // One query block per wave, pipelined over the tiles: the score product of tile t + 1 runs beside the exponentials of tile t, the
         // maximum of t + 1 beside the second product of t (LDS holds K of t + 1 and V of t while K of t + 2 and V of t + 1 arrive).
         auto kbuf = [&](int t) { return smem + (t & 1) * K_BYTES; };
@@ -522,54 +530,51 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
             }
         }
     } else {
-        // Two query blocks per wave, offset against each other within the tile: the score product of the second runs beside the
-        // exponentials of the first, the second product of the first beside the exponentials of the second.
-        // (8-bit keys: the next tile's codes are in registers meanwhile, and go into the other buffer at its end)
-        static_assert(!PAGED || KVM == 1, "one tile of codes at a time");
-        auto load = [&](int mt, char* dst) {
-#pragma unroll
-            for (int sub = 0; sub < KVM; ++sub) {
-                const int t = mt * KVM + sub;
-                if (t >= ktiles) break;
-                dma(false, t, dst + sub * TILE);
-                dma(true, t, dst + sub * TILE + K_BYTES);
+        // One tile at a time.  Two query blocks per wave are offset against each other within it: the score product of the second runs
+        // beside the exponentials of the first, the second product of the first beside the exponentials of the second.  (8-bit keys: the
+        // next tile's codes are in registers meanwhile, and go into the other buffer at its end.)
+        auto load = [&](int t, char* dst) {
+            dma(false, t, dst);
+            dma(true, t, dst + K_BYTES);
+        };
+        auto work = [&](int t, char* sK, char* sV) __attribute__((always_inline)) {
+            const bool edge = (t + 1) * 64 > w_first || (PAGED && have != 0xf);
+            f32x16 s0[2];
+            bf16x8 pf0[2][2];
+            qk(sK, 0, s0);
+            if (edge) mask(t, 0, s0, have);
+            raise_max(0, row_max(s0));
+            if constexpr (QB == 2) {
+                f32x16 s1[2];
+                bf16x8 pf1[2][2];
+                qk(sK, 1, s1);
+                exp_pack(0, s0, pf0);
+                pin(pf0);
+                if (edge) mask(t, 1, s1, have);
+                raise_max(1, row_max(s1));
+                pv(sV, 0, pf0);
+                exp_pack(1, s1, pf1);
+                pv(sV, 1, pf1);
+            } else {
+                exp_pack(0, s0, pf0);
+                pv(sV, 0, pf0);
             }
         };
-        auto step = [&](int mt, char* here, char* dst) {
+        auto step = [&](int t, char* here, char* dst) {
             if constexpr (PAGED) {
-                const int tk = min(mt + 1, t1 - 1);
+                const int tk = min(t + 1, t1 - 1);
                 fetch(false, tk, pid_k, k8r, kbyte);
                 fetch(true, tk, pid_k, v8r, vbyte);
                 have1 = groups(pid_k);
-                pid_k = look_up(min(mt + 2, t1 - 1));
+                pid_k = look_up(min(t + 2, t1 - 1));
             } else {
-                if (mt + 1 < t1) load(mt + 1, dst);
+                if (t + 1 < t1) load(t + 1, dst);
             }
-#pragma unroll
-            for (int sub = 0; sub < KVM; ++sub) {
-                const int t = mt * KVM + sub;
-                if (t >= ktiles) break;
-                char* sK = here + sub * TILE;
-                char* sV = sK + K_BYTES;
-                if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
-                    if (tile_nonfinite(sV)) absorb_nonfinite(sK, sV, t);
-                }
-                if (t * 64 >= w_last) continue;
-                const bool edge = (t + 1) * 64 > w_first || (PAGED && have != 0xf);
-                f32x16 s0[2], s1[2];
-                bf16x8 pf0[2][2], pf1[2][2];
-                qk(sK, 0, s0);
-                if (edge) mask(t, 0, s0, have);
-                raise_max(0, row_max(s0));
-                qk(sK, QB - 1, s1);
-                exp_pack(0, s0, pf0);
-                pin(pf0);
-                if (edge) mask(t, QB - 1, s1, have);
-                raise_max(QB - 1, row_max(s1));
-                pv(sV, 0, pf0);
-                exp_pack(QB - 1, s1, pf1);
-                pv(sV, QB - 1, pf1);
+            char* sV = here + K_BYTES;
+            if ((t + 1) * 64 > wg_first || (PAGED && have != 0xf)) {
+                if (tile_nonfinite(sV)) absorb_nonfinite(here, sV, t);
             }
+            if (t * 64 < w_last) work(t, here, sV);
             if constexpr (PAGED) {
                 stage_k(dst);
                 stage_v(dst + K_BYTES);
@@ -578,7 +583,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
             arrive();
         };
         if (t0 < t1) {
-            char* first = smem + (t0 & 1) * BUF;
+            char* first = smem + (t0 & 1) * TILE;
             if constexpr (PAGED) {
                 const int pid = look_up(t0);
                 pid_k = look_up(min(t0 + 1, t1 - 1));
@@ -591,7 +596,7 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
                 load(t0, first);
             }
             arrive();
-            for (int mt = t0; mt < t1; ++mt) step(mt, smem + (mt & 1) * BUF, smem + (1 - (mt & 1)) * BUF);
+            for (int t = t0; t < t1; ++t) step(t, smem + (t & 1) * TILE, smem + (1 - (t & 1)) * TILE);
         }
     }
 
@@ -633,23 +638,23 @@ __global__ __launch_bounds__(64 * NW, 2) void seq_attn_tile_kernel(const SeqAttn
     }
 }
 
-template <int D, int QB, int NW, int KVM, int FMT, bool PAGED>
+template <int D, int QB, int NW, int FMT, bool PAGED>
 int launch(const SeqAttnParams& p_in, hipStream_t stream) {
     SeqAttnParams p = p_in;
     constexpr int BM = 32 * NW * QB;
     p.qtiles = (int)(((long)p.max_q * p.G + BM - 1) / BM);
     const long n = (long)p.qtiles * p.splits * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
-    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, KVM, FMT, PAGED>), dim3((unsigned)n), dim3(64 * NW), 0, stream, p);
+    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, FMT, PAGED>), dim3((unsigned)n), dim3(64 * NW), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
 }
 
 template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
-    if (small) return D == 64 ? launch<64, 1, 4, 1, FMT, PAGED>(p, stream) : launch<128, 1, 4, 1, FMT, PAGED>(p, stream);
-    if constexpr (PAGED) return D == 64 ? launch<64, 2, 4, 1, FMT, PAGED>(p, stream) : launch<128, 1, 8, 1, FMT, PAGED>(p, stream);
-    else return launch<64, 2, 4, 2, FMT, PAGED>(p, stream);
+    if (small) return D == 64 ? launch<64, 1, 4, FMT, PAGED>(p, stream) : launch<128, 1, 4, FMT, PAGED>(p, stream);
+    if constexpr (PAGED) return D == 64 ? launch<64, 2, 4, FMT, PAGED>(p, stream) : launch<128, 1, 8, FMT, PAGED>(p, stream);
+    else return launch<64, 1, 8, FMT, PAGED>(p, stream);
 }
 
 }  // namespace
@@ -660,23 +665,25 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
 }
 
 // Tile height and key ranges.  128-row tiles (four waves), but
-//   16-bit keys, head dim 64: 256 rows (two query blocks per wave) where they fill the chip twice;
+//   16-bit keys, head dim 64: 256 rows (eight waves) where they fill the chip twice (4 x 2 748 tokens, 16 heads, full: 171 -> 164 us, 2 x
+//   5 496 332 -> 309, but causal 8 x 1 374: 55 -> 57);
 //   8-bit keys: the workgroup converts the keys it reads, half of that work per row for 256 rows.  Head dim 128 (eight waves, whose
 //   coupling costs less than that: 1 374 rows against 10 175 tokens, 5 x 8 heads: 540 -> 420 us; with 16-bit keys 974 -> 1 033): more
 //   than 128 rows.  Head dim 64 (two query blocks per wave: 1 374 rows, 6 x 8 heads, 36 343 tokens 590 -> 525 us; 2 x 16 heads, 12 366
 //   tokens 250 -> 237; but 3 x 16 heads, 1 374 tokens, causal 33 -> 47, 4 heads, 2 748 tokens 24 -> 31): where the estimate below is lower.
-// Ranges, where the grid is small: the work of all items over the CUs (two run together on one, a CU with a single item has 0.55 of
-// the rate; with n per CU the last to finish has between n and ceil(n)), half of an item for the tail, and the fold (a launch of 3 us;
-// 4 D bytes per row and range written and read), in microseconds at the rates measured here (a CU does `rate` flop in one; causal
-// masks, unknown here, count for 0.7).  192 items of 256 rows, 12 366 tokens, tile kernel: 265 us in 2 ranges, 271 in 3, 233 in 4, 237 in
-// 5, 245 in 6, 235 in 8; with n + 1/2 in place of the mean of n and ceil(n) it took 6.
+// Ranges, where the grid is small: the time of all items over the CUs, where the last CU to finish has between n and ceil(n) of n per CU
+// (one alone runs at 0.8 of a full CU's rate, at head dim 64 two at 0.9 of it), half of an item for start and tail, and the fold (5 us,
+// and 4 D bytes per row and range written and read), in microseconds at the rates measured here (a CU does `rate` flop in one; causal
+// masks, unknown here, count for 0.7).  Measured: 192 items of 256 rows, 12 366 8-bit keys of 64: 265 us in 2 ranges, 271 in 3, 233 in 4,
+// 237 in 5, 245 in 6, 235 in 8; 176 items of 128 rows, 1 374 keys of 128: 37 unsplit, 42 in 2, 51 in 3; of 64: 28, 29, 29; 344 items, 2 748
+// keys of 64: 64, 61, 67; 285 causal items, 2 305 keys of 64: 42, 36.
 static SeqPlan ranges_of(int bm, double rate, long pairs, long rows, long max_k, int D, double& us) {
     const long items = pairs * ((rows + bm - 1) / bm), cus = 256;
-    const double item_us = 4.0 * D * bm * max_k / rate, fold_us = 8.0 * D * pairs * rows / 4.0e6;
+    const double item_us = 4.0 * D * bm * max_k / rate, fold_us = 8.0 * D * pairs * rows / (D == 64 ? 5.3e6 : 4.0e6);
     auto cost = [&](long s) {
         const double n = (double)items * s / cus;
-        const double alone = 1.0 / 0.55, even = 0.5 * (n + std::ceil(n)) + 0.1, busy = even > alone ? even : alone;
-        return item_us * (0.7 * busy + 0.5) / s + (s > 1 ? 3.0 + fold_us * s : 0.0);
+        const double least = D == 128 || n <= 1.0 ? 1.25 : 1.8, even = 0.5 * (n + std::ceil(n)) + 0.1, busy = even > least ? even : least;
+        return item_us * (0.7 * busy + 0.5) / s + (s > 1 ? 5.0 + fold_us * s : 0.0);
     };
     SeqPlan plan = {1, bm == 128, 0};
     us = cost(1);
