@@ -503,8 +503,8 @@ int iggt_hdbscan_labels_from_mst(const int* eu, const int* ev, const float* ew, 
  * contiguous, q / k / v 16-byte and o 8-byte aligned; D = 64 | 128; query head h reads key head h / (Hq / Hkv).  Sequence b is
  * rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] .. cu_k[b + 1] (int32 on the device, clamped to the tensors); max_q / max_k bound the
  * lengths from above (rows past max_q of a sequence are not computed; max_k only chooses the number of key ranges).  Rows of o
- * outside the sequences are left as they are.  scale > 0.  ws: scratch of at least ..._ws_bytes (0: none needed), 16-byte
- * aligned, for this call alone while it runs. */
+ * outside the sequences are left as they are.  0 < scale <= 1e38; Tq * Hq < 2^31.  o may be q itself, and must not overlap the inputs
+ * in another way.  ws: scratch of at least ..._ws_bytes (0: none needed), 16-byte aligned, for this call alone while it runs. */
 long iggt_packed_attn_ws_bytes(int B, int max_q, int max_k, int Hq, int Hkv, int D);
 int iggt_packed_attn_bf16(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs,
                           long v_hs, void* o, long o_rs, long o_hs, const int* cu_q, const int* cu_k, int B, int Tq, int Tk,
