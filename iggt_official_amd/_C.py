@@ -14,7 +14,7 @@ _LIB_PATH = os.environ.get("IGGT_HIP_LIB") or os.path.join(os.path.dirname(os.pa
                                                            "libiggt_hip.so")
 _lib = None
 
-ABI_VERSION = 28
+ABI_VERSION = 29
 
 _c_void_p, _c_int, _c_long, _c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 
@@ -145,6 +145,7 @@ _SIGNATURES = {
     "iggt_append_pages_f16": [_c_void_p, _c_long, _c_long] * 2 + [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 4 + [_c_void_p],
     "iggt_plan_pages": [_c_void_p, _c_long, _c_int, _c_int, _c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 4
                        + [_c_int, _c_void_p],
+    "iggt_seq_attn_plan": [_c_int] * 7 + [ctypes.POINTER(_c_int)] * 2,
     "iggt_seq_call": [ctypes.c_char_p],
 }
 

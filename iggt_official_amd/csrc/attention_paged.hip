@@ -472,6 +472,14 @@ static int paged_attn_h16(int fmt, const void* q, long q_rs, long q_hs, void* o,
 }
 
 extern "C" {
+int iggt_seq_attn_plan(int paged, int B, int max_q, int max_k, int Hq, int Hkv, int D, int* rows, int* ranges) {
+    if (B <= 0 || max_q <= 0 || max_k < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return -1;
+    const int G = Hq / Hkv;
+    const SeqPlan plan = paged ? paged_plan(B, max_q, max_k, Hkv, G, D) : iggt_seq_tile_plan(B, max_q, max_k, Hkv, G, D, false);
+    *rows = paged && few_rows(B, max_q, max_k, Hkv, G) ? 16 : (plan.small ? 128 : 256);
+    *ranges = plan.splits;
+    return 0;
+}
 long iggt_paged_attn_ws_bytes(int B, int max_q, int max_len, int Hq, int Hkv, int D) {
     if (B <= 0 || max_q <= 0 || max_len < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128)) return 0;
     const SeqPlan plan = paged_plan(B, max_q, max_len, Hkv, Hq / Hkv, D);
