@@ -111,9 +111,8 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
     const long rows = (long)sp.lq * p.G;
     const long row0 = (long)qt * BM;
     if (row0 >= rows) return;
-    const int off = sp.lk - sp.lq;
     auto limit_of = [&](long row) {   // keys that row sees
-        return p.causal ? max(min(sp.lk, off + (int)(row / p.G) + 1), 0) : sp.lk;
+        return p.causal ? max(min(sp.lk, sp.off + (int)(row / p.G) + 1), 0) : sp.lk;
     };
     const int kend = limit_of(min(row0 + BM, rows) - 1);
     const int ktiles = (kend + 63) >> 6;

@@ -47,15 +47,15 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
     const SeqSpan sp = seq_span<true>(p, b);
     const int rows = min(sp.lq * p.G - row0, 16);
     if (rows <= 0) return;
-    const int off = sp.lk - sp.lq;
-    const int kend = sp.lk;
-    const int first = p.causal ? max(min(sp.lk, off + row0 / p.G + 1), 0) : sp.lk;    // keys that every row sees
+    const int first = p.causal ? max(min(sp.lk, sp.off + row0 / p.G + 1), 0) : sp.lk;    // keys that every row sees
+    // keys that some row sees (one token: the same)
+    const int kend = !DRAFT ? first : (p.causal ? max(min(sp.lk, sp.off + (row0 + rows - 1) / p.G + 1), 0) : sp.lk);
     // key range of the work item: whole rounds of the four waves (256 keys), of the same length for every request
     const int b0 = split * p.range_blocks;
     const int b1 = split == p.splits - 1 ? (kend + 63) >> 6 : min(b0 + p.range_blocks, (kend + 63) >> 6);   // (max_len may be too small)
 
     const int rn = row0 + min(n, rows - 1), qi = rn / p.G, hq = h * p.G + rn - qi * p.G;
-    const int lim = p.causal ? max(min(sp.lk, off + qi + 1), 0) : sp.lk;
+    const int lim = p.causal ? max(min(sp.lk, sp.off + qi + 1), 0) : sp.lk;
     bf16x8 qf[NC][2];
     {
         const bf16_t* src = p.q + (long)(sp.q0 + qi) * p.q_rs + (long)hq * p.q_hs + 16 * g;
@@ -162,8 +162,8 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
             l += e[j];
         }
         const bf16x8 p0 = pack8f<FMT>(e), p1 = pack8f<FMT>(e + 8);
-        // codes 0x7f / 0xff are NaN (e4m3 has no infinity) and 0 * NaN is one: what lies behind the last key (whatever the page held) is
-        // zeroed, what only some rows see is found here
+        // codes 0x7f / 0xff are NaN (e4m3 has no infinity) and 0 * NaN is one: what lies behind the last key that a row sees (whatever the
+        // page holds there) is zeroed, what only some rows see is found here
         bool bad = false;
         if (edge) {
             const int held = !page_ok(p, here) ? 0 : kend - key0;
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams 
     const long row = (long)blockIdx.x * (4 / W) + wave / W;    // ((b, token), head)
     const long per = (long)p.max_q * p.Hq;
     const int b = (int)(row / per);
-    SeqSpan sp = {0, 0, 0, 0};
+    SeqSpan sp = {0, 0, 0, 0, 0};
     if (b < p.B) sp = seq_span<PAGED>(p, b);
     const int i = (int)((row - b * per) / p.Hq), hq = (int)(row % p.Hq);
     const bool live = b < p.B && i < sp.lq;

@@ -44,8 +44,10 @@ constexpr float P_SHIFT_F16 = 8.0f;  // fp16 numerators are 2^(s - m + 8): the s
 
 struct SeqSpan {
     int q0, lq, lk, k0;
+    int off;              // causal: row i sees keys j <= i + off
 };
-// Rows and keys of sequence b.  The prefix sums and lengths are device data nobody has checked: they are clamped to the tensors.
+// Rows and keys of sequence b.  The prefix sums and lengths are device data nobody has checked: they are clamped to the tensors.  lq is
+// the number of rows to compute (max_q at most), off that of the whole sequence.
 template <bool PAGED>
 IGGT_DEVINL SeqSpan seq_span(const SeqAttnParams& p, int b) {
     SeqSpan s;
@@ -57,7 +59,8 @@ IGGT_DEVINL SeqSpan seq_span(const SeqAttnParams& p, int b) {
         s.q0 = min(b, p.Tq);
         q1 = min(b + 1, p.Tq);
     }
-    s.lq = min(max(q1 - s.q0, 0), p.max_q);
+    const int lq = max(q1 - s.q0, 0);
+    s.lq = min(lq, p.max_q);
     if constexpr (PAGED) {
         s.k0 = 0;
         s.lk = (int)min((long)max(p.lens[b], 0), (long)p.table_width << p.page_shift);
@@ -65,6 +68,7 @@ IGGT_DEVINL SeqSpan seq_span(const SeqAttnParams& p, int b) {
         s.k0 = min(max(p.cu_k[b], 0), p.Tk);
         s.lk = max(min(max(p.cu_k[b + 1], 0), p.Tk) - s.k0, 0);
     }
+    s.off = s.lk - lq;
     return s;
 }
 

@@ -502,7 +502,8 @@ int iggt_hdbscan_labels_from_mst(const int* eu, const int* ev, const float* ew, 
  * q / o: 16-bit [Tq][Hq][D], k / v: 16-bit [Tk][Hkv][D], row and head strides in elements (multiples of 8, o: of 4), channels
  * contiguous, q / k / v 16-byte and o 8-byte aligned; D = 64 | 128; query head h reads key head h / (Hq / Hkv).  Sequence b is
  * rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] .. cu_k[b + 1] (int32 on the device, clamped to the tensors); max_q / max_k bound the
- * lengths from above (rows past max_q of a sequence are not computed; max_k only chooses the number of key ranges).  Rows of o
+ * lengths from above (of a longer sequence the first max_q rows are computed, under the whole one's mask; max_k only chooses the number
+ * of key ranges).  Rows of o
  * outside the sequences are left as they are.  0 < scale <= 1e38; Tq * Hq < 2^31.  o may be q itself, and must not overlap the inputs
  * in another way.  ws: scratch of at least ..._ws_bytes (0: none needed), 16-byte aligned, for this call alone while it runs. */
 long iggt_packed_attn_ws_bytes(int B, int max_q, int max_k, int Hq, int Hkv, int D);

@@ -1,0 +1,52 @@
+"""Packed and cached attention at the borders of what their documentation allows, against the 64-bit references of packed_ref.py."""
+import pytest
+import torch
+
+import packed_ref as R
+from iggt_official_amd.layers import Pages, append_pages, packed_attention, paged_attention
+from test_packed_gpu import INF, NAN, ints, make_cache, rand
+from test_packed_paths_gpu import cached, plan
+
+pytestmark = pytest.mark.gpu
+
+
+def first_rows(lq, max_q):
+    """Mask over the packed rows: the first max_q of every sequence."""
+    return torch.cat([torch.arange(n) < max_q for n in lq]).cuda()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,hq,hkv,lq,lk,max_q,item", [
+    (64, 2, 2, [64], [64], 10, 128), (128, 4, 1, [64, 5, 30], [64, 40, 12], 10, 128), (64, 16, 16, [400] * 40, [400] * 40, 270, 256),
+    (64, 1, 1, [900], [5000], 130, 128), (128, 2, 2, [3], [6000], 1, 128)])
+def test_packed_rows_behind_max_q_do_not_move_the_mask(dim, hq, hkv, lq, lk, max_q, item, dt):
+    """Of a sequence longer than max_q the first rows are computed, under the mask of the whole sequence; the others stay as they are."""
+    assert plan(False, len(lq), max_q, max(lk), hq, hkv, dim)[0] == item
+    q, k, v = rand((sum(lq), hq, dim), 1, R.H16[dt]), rand((sum(lk), hkv, dim), 2, R.H16[dt]), rand((sum(lk), hkv, dim), 3, R.H16[dt])
+    v[lk[0] - 1] = NAN                               # only the last row of the first sequence sees it
+    few = first_rows(lq, max_q)
+    out = torch.full_like(q, 3.0)
+    packed_attention(q, k, v, R.starts(lq, "cuda"), R.starts(lk, "cuda"), max_q, max(lk), out=out)
+    ref, tol = R.attention(q, k, v, lq, lk, True)
+    R.close(out[few], ref[few], tol[few])
+    assert (out[~few] == 3).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,hq,hkv,lq,lens,max_q,item", [
+    (64, 4, 2, [3, 9, 1, 0], [70, 200, 20, 9], 1, 16), (128, 4, 4, [30, 9], [300, 200], 2, 16), (64, 2, 1, [64], [64], 10, 16), (128, 1, 1, [40], [6000], 1, 16),
+    (64, 4, 2, [200, 300], [250, 300], 150, 128), (64, 32, 32, [150] * 16, [200] * 16, 130, 256), (128, 4, 2, [200, 300], [250, 300], 150, 256),
+    (128, 1, 1, [150], [5000], 100, 128)])
+def test_cached_rows_behind_max_q_do_not_move_the_mask(dim, hq, hkv, lq, lens, max_q, item, dt):
+    assert plan(True, len(lq), max_q, max(lens), hq, hkv, dim)[0] == item
+    pages, tables = make_cache(lens, 16, hkv, dim, 4)
+    last = lens[0] - 1                               # a NaN that only the last row of the first request sees
+    pages.v_codes[int(tables[0, last // 16]), 0, 0, 7, last % 16] = 0x7f
+    q = rand((sum(lq), hq, dim), 5, R.H16[dt])
+    few = first_rows(lq, max_q)
+    out = torch.full_like(q, 3.0)
+    cached(q, pages, tables, lens, lq, max_q=max_q, out=out)
+    k, v = R.held(pages, tables, lens)
+    ref, tol = R.attention(q, k, v, lq, lens, True)
+    R.close(out[few], ref[few], tol[few])
+    assert (out[~few] == 3).all()
