@@ -182,22 +182,20 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
     // fp16 holds half of each value (a code of a scale near fp16's range would round to 2^16): the factor 2 of K goes into the softmax
     // scale, that of V into the epilogue.
     constexpr int PIECES = 4 * D;                                       // 16-byte pieces of K in a tile, and of V
-    constexpr int PPT = PIECES > NT ? PIECES / NT : 1;                  // a thread's of each
-    constexpr bool APART = PIECES < NT;                                 // the first half of the waves takes K, the second V
+    constexpr int PPT = PIECES / NT;                                    // a thread's of each
+    static_assert(!PAGED || PIECES % NT == 0, "every thread takes as many");
     constexpr float HALF = (PAGED && FMT == FMT_F16) ? 0.5f : 1.0f;
-    u32x4 k8r[PPT], v8r[PPT];
-    uint32_t kbyte[PPT], vbyte[PPT];
+    constexpr int HELD = PPT > 0 ? PPT : 1;                             // (16-bit keys: nothing)
+    u32x4 k8r[HELD], v8r[HELD];
+    uint32_t kbyte[HELD], vbyte[HELD];
     uint32_t have = 0xf, have1 = 0xf, have2 = 0xf;   // which 16-key groups have a page: this tile, the next one, the one after it
     // a wave's piece i lies in one 16-key group of D pieces: one table entry (lane l: group l & 3), loaded a tile ahead, serves its K
     // and, a tile later, its V
-    const int first_piece = APART ? tid & (PIECES - 1) : tid;
-    const int psub = __builtin_amdgcn_readfirstlane(first_piece / D), pin16 = first_piece % D;   // group (+ i NT / D) and piece within it
-    const bool takes_k = !APART || wave < NW / 2, takes_v = !APART || wave >= NW / 2;
+    const int psub = __builtin_amdgcn_readfirstlane(tid / D), pin16 = tid % D;   // group (+ i NT / D) and piece within it
     int pid_v = 0, pid_k = 0;
     auto look_up = [&](int t) { return page_entry(p, b, t * 64 + (lane & 3) * 16); };
     auto groups = [&](int pid) { return (uint32_t)__ballot(page_ok(p, pid)) & 0xfu; };
-    auto fetch = [&](bool V, int t, int pid, u32x4 (&code)[PPT], uint32_t (&byte)[PPT]) {
-        if (V ? !takes_v : !takes_k) return;
+    auto fetch = [&](bool V, int t, int pid, u32x4 (&code)[HELD], uint32_t (&byte)[HELD]) {
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
             const int sub = psub + i * (NT / D), id = __builtin_amdgcn_readlane(pid, sub);
@@ -208,7 +206,6 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
         }
     };
     auto stage_k = [&](char* sK) {
-        if (!takes_k) return;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
             const int key = (psub + i * (NT / D)) * 16 + pin16 / (D / 16), piece = pin16 % (D / 16), sw = D == 64 ? (key >> 1) & 7 : key & 15;
@@ -219,7 +216,6 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
         }
     };
     auto stage_v = [&](char* sV) {
-        if (!takes_v) return;
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
             const int sub = psub + i * (NT / D);
@@ -653,7 +649,7 @@ template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
     if (small) return D == 64 ? launch<64, 1, 4, FMT, PAGED>(p, stream) : launch<128, 1, 4, FMT, PAGED>(p, stream);
     if constexpr (PAGED) return D == 64 ? launch<64, 2, 4, FMT, PAGED>(p, stream) : launch<128, 1, 8, FMT, PAGED>(p, stream);
-    else return launch<64, 1, 8, FMT, PAGED>(p, stream);
+    else return D == 64 ? launch<64, 1, 8, FMT, PAGED>(p, stream) : -1;    // (the plan has 128-row tiles for 128 channels)
 }
 
 }  // namespace
