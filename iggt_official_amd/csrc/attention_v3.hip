@@ -420,8 +420,8 @@ __global__ __launch_bounds__(256, 2) void flash_attn_d64_v3_kernel(const AttnPar
 #pragma unroll
         for (int kvh = 0; kvh < 2; ++kvh) {
             if (decltype(use_delta)::value && qb == 1) {
-                // the accumulator holds s - c + SHIFT with c of the FIRST block's row: move to this row's shift, two scores per
-                // v_pk_add_f32 (written as scalar subtractions the compiler emitted 32 v_sub_f32 per tile)
+                // the accumulator holds s - c + SHIFT with c of the FIRST block's row: move to this row's shift (in pairs, for the
+                // order of instructions that was measured; the library is built without packed fp32, so these are 32 v_sub_f32 a tile)
                 typedef float f32x2 __attribute__((ext_vector_type(2)));
                 const f32x2 d2 = {est_delta, est_delta};
 #pragma unroll
