@@ -179,8 +179,10 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
     };
     // 8-bit: codes go through registers (16 bytes each), are converted and written as 16-bit tiles: K rows like above, V transposed
     // [D][64 keys] with the keys of every 16 in the order 0-3, 8-11 | 4-7, 12-15 (what the two lane halves need side by side).
-    // fp16 holds half of each value (a code of a scale near fp16's range would round to 2^16): the factor 2 of K goes into the softmax
-    // scale, that of V into the epilogue.
+    // fp16 holds half of V's values (a code of a scale near fp16's range would round to 2^16; the factor 2 goes into the epilogue), and
+    // K's times a power of two that takes the largest scale of the key range to 2^7 (a cache may have been written from bf16; the inverse
+    // goes into the softmax scale): exact for scales down to 2^-15, 22 powers of two below the largest, and a key that is smaller yet is
+    // off by 2^-42 of the largest key.
     constexpr int PIECES = 4 * D;                                       // 16-byte pieces of K in a tile, and of V
     constexpr int PPT = PIECES / NT;                                    // a thread's of each
     static_assert(!PAGED || PIECES % NT == 0, "every thread takes as many");
@@ -205,12 +207,33 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
             code[i] = *reinterpret_cast<const u32x4*>((V ? p.v8 : p.k8) + at);
         }
     };
+    float kf = 1.0f, c = p.scale_log2;
+    if constexpr (PAGED && FMT == FMT_F16) {
+        __shared__ int s_top[NW];
+        int top = 7;                                 // (the factor stays a float)
+        const int pages = ((min(t1 * 64, kend) - 1) >> p.page_shift) + 1;
+        for (int i = ((t0 * 64) >> p.page_shift) + tid; i < pages; i += NT) {
+            const int id = page_entry(p, b, i << p.page_shift);
+            if (page_ok(p, id)) top = max(top, (int)p.k_scale[(long)id * p.Hkv + h]);
+        }
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) top = max(top, __shfl_xor(top, x, 64));
+        if (lane == 0) s_top[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) top = max(top, s_top[w]);
+        const int shift = 134 - __builtin_amdgcn_readfirstlane(min(top, 254));
+        kf = __builtin_bit_cast(float, (127 + shift) << 23);
+        // (neither 0 nor inf, times which a masked score or a zero would be NaN)
+        c = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(c, -shift), 0x1p-149f, 3.4028235e38f);
+        c = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, c)));
+    }
     auto stage_k = [&](char* sK) {
 #pragma unroll
         for (int i = 0; i < PPT; ++i) {
             const int key = (psub + i * (NT / D)) * 16 + pin16 / (D / 16), piece = pin16 % (D / 16), sw = D == 64 ? (key >> 1) & 7 : key & 15;
             bf16x8 lo, hi;
-            cvt16<FMT>(k8r[i], scale_of(kbyte[i]) * HALF, lo, hi);
+            cvt16<FMT>(k8r[i], scale_of(kbyte[i]) * kf, lo, hi);
             *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece) ^ sw) * 16) = lo;
             *reinterpret_cast<bf16x8*>(sK + key * ROWB + ((2 * piece + 1) ^ sw) * 16) = hi;
         }
@@ -239,7 +262,6 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[qb][dh][r] = 0.f;
     }
-    const float c = p.scale_log2 * (PAGED && FMT == FMT_F16 ? 2.f : 1.f);
 
     // lane-dependent LDS offsets
     int koff[NKC], voff[NDH];

@@ -50,3 +50,25 @@ def test_cached_rows_behind_max_q_do_not_move_the_mask(dim, hq, hkv, lq, lens, m
     ref, tol = R.attention(q, k, v, lq, lens, True)
     R.close(out[few], ref[few], tol[few])
     assert (out[~few] == 3).all()
+
+
+KERNELS = pytest.mark.parametrize("item,dim,heads,rows", [(16, 64, 1, 20), (16, 128, 1, 1), (128, 64, 1, 200), (256, 64, 512, 130), (256, 128, 1, 200), (128, 128, 16, 100)])
+
+
+@pytest.mark.parametrize("size,of_q,scale", [(1e6, 1e-5, None), (1e-6, 3e4, 4.0), (3e-8, 3e4, 120.0)])
+@KERNELS
+def test_fp16_rows_over_keys_beyond_the_range_of_fp16(item, dim, heads, rows, size, of_q, scale):
+    """A cache written from bf16 holds keys that fp16 does not: their scores are formed from the codes, the scale goes on in fp32."""
+    n = 4200 if (item, dim) == (128, 128) else 190
+    assert plan(True, 1, rows, n, heads, heads, dim)[0] == item
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = (torch.randn(n, heads, dim, device="cuda", generator=g) * size).bfloat16()
+    k[16:32] *= 0.25                                 # (pages of other scales beside them)
+    v = rand((n, heads, dim), 4, torch.bfloat16)
+    pages = Pages.empty(-(-n // 16), heads, dim, 16)
+    append_pages(pages, k, v, torch.arange(n, dtype=torch.int32, device="cuda"))
+    tables = torch.arange(-(-n // 16), dtype=torch.int32, device="cuda")[None]
+    q = (torch.randn(rows, heads, dim, device="cuda", generator=g).clamp(-2, 2) * of_q).half()
+    kk, vv = R.held(pages, tables, [n])
+    for causal in (True, False):
+        R.close(cached(q, pages, tables, [n], [rows], causal, scale=scale), *R.attention(q, kk, vv, [rows], [n], causal, scale=scale))
