@@ -294,9 +294,11 @@ __global__ __launch_bounds__(256) void seq_attn_fold_kernel(const SeqAttnParams 
         for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
         const float weight = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
         total = wave_sum(l * weight);
+        // (a range without a key has left no sum; one whose weight vanishes counts with 0, so that its infinities and NaN do not get lost)
+        const unsigned long long some = __ballot(l != 0.f);
         for (int s = (wave % W) * NG; s < p.splits; s += NG * W) {
-            const float f = __shfl(weight, s + gr, 64);      // 0 behind the last range
-            if (f != 0.f) acc += *reinterpret_cast<const f32x4*>(p.part_o + ((s + gr) * step + row) * D + d) * f;
+            const float f = __shfl(weight, s + gr, 64);
+            if ((some >> (s + gr)) & 1) acc += *reinterpret_cast<const f32x4*>(p.part_o + ((s + gr) * step + row) * D + d) * f;
         }
 #pragma unroll
         for (int x = LPR; x < 64; x *= 2)

@@ -72,3 +72,24 @@ def test_fp16_rows_over_keys_beyond_the_range_of_fp16(item, dim, heads, rows, si
     kk, vv = R.held(pages, tables, [n])
     for causal in (True, False):
         R.close(cached(q, pages, tables, [n], [rows], causal, scale=scale), *R.attention(q, kk, vv, [rows], [n], causal, scale=scale))
+
+
+@pytest.mark.parametrize("paged,rows,lk", [(True, 1, 2000), (True, 1, 20000), (True, 5, 2000), (True, 5, 20000), (True, 200, 20000), (False, 1, 2000), (False, 1, 20000)])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_nan_in_a_key_range_whose_weight_vanishes(paged, rows, lk, dim, dt):
+    """One key outweighs all others by 2^250: a NaN among those still reaches the rows that see it, whatever number of key ranges there is."""
+    q, k, v = rand((rows, 1, dim), 1, R.H16[dt], 0.1), rand((lk, 1, dim), 2, R.H16[dt], 0.1), rand((lk, 1, dim), 3, R.H16[dt])
+    q[:, :, 0], k[:, :, 0] = 16.0, 0.0
+    k[5, 0, 0] = 192.0 / 16 * dim ** 0.5
+    v[lk // 2 + 9, 0, 11] = NAN
+    if paged:
+        pages = Pages.empty(-(-lk // 64), 1, dim, 64)
+        append_pages(pages, k, v, torch.arange(lk, dtype=torch.int32, device="cuda"))
+        tables = torch.arange(-(-lk // 64), dtype=torch.int32, device="cuda")[None]
+        o = cached(q, pages, tables, [lk], [rows])
+        k, v = R.held(pages, tables, [lk])
+    else:
+        o = packed_attention(q, k, v, R.starts([rows], "cuda"), R.starts([lk], "cuda"), rows, lk)
+    assert (plan(paged, 1, rows, lk, 1, 1, dim)[1] > 8) == (lk == 20000)
+    R.close(o, *R.attention(q, k, v, [rows], [lk], True))
