@@ -162,8 +162,8 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
             l += e[j];
         }
         const bf16x8 p0 = pack8f<FMT>(e), p1 = pack8f<FMT>(e + 8);
-        // codes 0x7f / 0xff are NaN (e4m3 has no infinity) and 0 * NaN is one: what lies behind the last key that a row sees (whatever the
-        // page holds there) is zeroed, what only some rows see is found here
+        // 0 * NaN and 0 * inf are NaN: what lies behind the last key that a row sees (whatever the page holds there) is zeroed, and what only
+        // some rows see is looked for here -- codes 0x7f / 0xff (NaN; e4m3 has no infinity), and scales at which fp16 does not hold 448
         bool bad = false;
         if (edge) {
             const int held = !page_ok(p, here) ? 0 : kend - key0;
@@ -179,6 +179,7 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
                 }
                 if (DRAFT) bad = bad || nan != 0;
             }
+            if (DRAFT && FMT == FMT_F16) bad = bad || (vs > 128.f && held > 0);
             if (DRAFT) bad = __any(bad);
         }
         if (!DRAFT || !bad) {
@@ -190,31 +191,38 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
                 o[i] = mfma16h<FMT>(hi, p1, o[i]);
             }
         } else {
-            // the product runs on zeros in their place, and a second one of 0 / 1 codes with the mask finds the rows that see one
+            // the product runs on zeros in the place of values that are not finite; further ones, of 1 where such a value is not negative
+            // and of 1 where it is (a NaN: both) with the mask, find the rows that see one
             float one[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) one[j] = j < seen ? 1.f : 0.f;
             const bf16x8 i0 = pack8f<FMT>(one), i1 = pack8f<FMT>(one + 8);
 #pragma unroll
             for (int i = 0; i < NDT; ++i) {
-                u32x4 nan;
+                bf16x8 v[2];
+                cvt16<FMT>(vc[i], vs, v[0], v[1]);
+                f32x4 plus = {0.f, 0.f, 0.f, 0.f}, minus = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    nan[w] = ((((vc[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
-                    vc[i][w] &= ~nan[w];
-                    nan[w] &= 0x38383838u;   // 1.0
+                for (int u = 0; u < 2; ++u) {
+                    constexpr uint32_t M = FMT == FMT_F16 ? 0x03ff03ffu : 0x007f007fu, ONE = FMT == FMT_F16 ? 0x3c003c00u : 0x3f803f80u;
+                    u32x4 w = __builtin_bit_cast(u32x4, v[u]), up, down;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t odd = nonfinite2<FMT>(w[j]);                                  // bits 15 and 31
+                        const uint32_t nan = odd & (((w[j] & M) + M) << (FMT == FMT_F16 ? 5 : 8));   // mantissa not 0
+                        up[j] = (((odd & ~w[j]) | nan) >> 15) * 0xffffu & ONE;
+                        down[j] = (((odd & w[j]) | nan) >> 15) * 0xffffu & ONE;
+                        w[j] &= ~((odd >> 15) * 0xffffu);
+                    }
+                    plus = mfma16h<FMT>(__builtin_bit_cast(bf16x8, up), u ? i1 : i0, plus);
+                    minus = mfma16h<FMT>(__builtin_bit_cast(bf16x8, down), u ? i1 : i0, minus);
+                    o[i] = mfma16h<FMT>(__builtin_bit_cast(bf16x8, w), u ? p1 : p0, o[i]);
                 }
-                bf16x8 lo, hi;
-                f32x4 cnt = {0.f, 0.f, 0.f, 0.f};
-                cvt16<FMT>(nan, 1.0f, lo, hi);
-                cnt = mfma16h<FMT>(lo, i0, cnt);
-                cnt = mfma16h<FMT>(hi, i1, cnt);
-                cvt16<FMT>(vc[i], vs, lo, hi);
-                o[i] = mfma16h<FMT>(lo, p0, o[i]);
-                o[i] = mfma16h<FMT>(hi, p1, o[i]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (cnt[r] > 0.f) o[i][r] = __builtin_nanf("");
+                for (int r = 0; r < 4; ++r) {
+                    if (plus[r] > 0.f) o[i][r] += INFINITY;
+                    if (minus[r] > 0.f) o[i][r] -= INFINITY;
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }

@@ -93,3 +93,20 @@ def test_nan_in_a_key_range_whose_weight_vanishes(paged, rows, lk, dim, dt):
         o = packed_attention(q, k, v, R.starts([rows], "cuda"), R.starts([lk], "cuda"), rows, lk)
     assert (plan(paged, 1, rows, lk, 1, 1, dim)[1] > 8) == (lk == 20000)
     R.close(o, *R.attention(q, k, v, [rows], [lk], True))
+
+
+@pytest.mark.parametrize("item,dim,heads,rows", [(16, 64, 2, 3), (16, 128, 1, 20), (128, 64, 1, 200), (256, 64, 512, 130), (256, 128, 1, 200)])
+def test_fp16_rows_over_values_beyond_the_range_of_fp16(item, dim, heads, rows):
+    """V beyond 131 008 is infinite for fp16 rows: for those that see it."""
+    n = 190
+    assert plan(True, 1, rows, n, heads, heads, dim)[0] == item
+    k, v = rand((n, heads, dim), 1, torch.bfloat16), rand((n, heads, dim), 2, torch.bfloat16)
+    v[n - 1, 0, 3], v[n - 1, 0, 4], v[n - 2, 0, 5], v[n - 2, 0, 6], v[n - 1, 0, 6], v[n - 2, 0, 7] = 4e5, -4e5, 3e5, 3e5, -3e5, NAN
+    pages = Pages.empty(12, heads, dim, 16)
+    append_pages(pages, k, v, torch.arange(n, dtype=torch.int32, device="cuda"))
+    tables = torch.arange(12, dtype=torch.int32, device="cuda")[None]
+    q = rand((rows, heads, dim), 3, torch.float16)
+    kk, vv = R.held(pages, tables, [n])
+    vv = torch.where(vv.abs() > 131008, vv.sign() * INF, vv)
+    for causal in (True, False):
+        R.close(cached(q, pages, tables, [n], [rows], causal), *R.attention(q, kk, vv, [rows], [n], causal))
