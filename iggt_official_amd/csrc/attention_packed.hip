@@ -740,7 +740,7 @@ static int packed_attn_h16(int fmt, const void* q, long q_rs, long q_hs, const v
     if (Tk >= 0x7fffffff - 1024 || (long)Tq * Hq >= (1L << 31)) return -1;
     if ((q_rs | q_hs | k_rs | k_hs | v_rs | v_hs) % 8 || (o_rs | o_hs) % 4) return -2;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || (uintptr_t)o % 8) return -2;
-    if (k_rs < 0 || v_rs < 0 || k_rs >= (1L << 24) || v_rs >= (1L << 24)) return -2;   // 64 rows in 32-bit byte offsets
+    if (Tk > 1 && (k_rs < 0 || v_rs < 0 || k_rs >= (1L << 24) || v_rs >= (1L << 24))) return -2;   // 64 rows in 32-bit byte offsets
     if (!(scale > 0.f && scale <= 1e38f)) return -3;
     if (B == 0 || Tq == 0 || max_q == 0) return 0;
     SeqAttnParams p = {};

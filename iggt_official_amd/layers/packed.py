@@ -111,8 +111,8 @@ def packed_attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, *, causal: boo
 
     max_q, max_k: the longest sequences' lengths or more (of a sequence with more rows the first max_q are computed, as they would be
     with all of them; max_k only steers how the work is split).  out: rows that belong to no sequence are left as they are; without it
-    they are 0.  It may be q itself, and must not overlap q in another way, nor k or v.  Prefix sums do not decrease: a row that two
-    sequences share has the values of either."""
+    they are 0.  It may be q itself, and must not overlap q in another way, nor k or v.  Rows of k and of v lie less than 2^24 elements
+    apart.  Prefix sums do not decrease: a row that two sequences share has the values of either."""
     where = q.get_device()
     if where < 0:
         _refuse("IGGT HIP ops need tensors on a ROCm device (no CPU fallback)")

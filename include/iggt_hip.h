@@ -499,13 +499,13 @@ int iggt_hdbscan_labels_from_mst(const int* eu, const int* ev, const float* ew, 
  *   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - m_i) / l_i  over the keys j of i's own sequence, with
  *   j <= i + Lk - Lq if causal (the last row sees the last key).  A row that sees no key is 0.
  *
- * q / o: 16-bit [Tq][Hq][D], k / v: 16-bit [Tk][Hkv][D], row and head strides in elements (multiples of 8, o: of 4), channels
- * contiguous, q / k / v 16-byte and o 8-byte aligned; D = 64 | 128; query head h reads key head h / (Hq / Hkv).  Sequence b is
- * rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] .. cu_k[b + 1] (int32 on the device, clamped to the tensors); max_q / max_k bound the
- * lengths from above (of a longer sequence the first max_q rows are computed, under the whole one's mask; max_k only chooses the number
- * of key ranges).  Rows of o
- * outside the sequences are left as they are.  0 < scale <= 1e38; Tq * Hq < 2^31.  o may be q itself, and must not overlap the inputs
- * in another way.  ws: scratch of at least ..._ws_bytes (0: none needed), 16-byte aligned, for this call alone while it runs. */
+ * q / o: 16-bit [Tq][Hq][D], k / v: 16-bit [Tk][Hkv][D], row and head strides in elements (multiples of 8, o: of 4; rows of k and of v
+ * less than 2^24 apart), channels contiguous, q / k / v 16-byte and o 8-byte aligned; D = 64 | 128; query head h reads key head
+ * h / (Hq / Hkv).  Sequence b is rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] .. cu_k[b + 1] (int32 on the device, clamped to the
+ * tensors); max_q / max_k bound the lengths from above (of a longer sequence the first max_q rows are computed, under the whole one's
+ * mask; max_k only chooses the number of key ranges).  Rows of o outside the sequences are left as they are.  0 < scale <= 1e38;
+ * Tq * Hq < 2^31.  o may be q itself, and must not overlap the inputs in another way.  ws: scratch of at least ..._ws_bytes (0: none
+ * needed), 16-byte aligned, for this call alone while it runs. */
 long iggt_packed_attn_ws_bytes(int B, int max_q, int max_k, int Hq, int Hkv, int D);
 int iggt_packed_attn_bf16(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs,
                           long v_hs, void* o, long o_rs, long o_hs, const int* cu_q, const int* cu_k, int B, int Tq, int Tk,

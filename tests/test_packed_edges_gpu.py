@@ -110,3 +110,14 @@ def test_fp16_rows_over_values_beyond_the_range_of_fp16(item, dim, heads, rows):
     vv = torch.where(vv.abs() > 131008, vv.sign() * INF, vv)
     for causal in (True, False):
         R.close(cached(q, pages, tables, [n], [rows], causal), *R.attention(q, kk, vv, [rows], [n], causal))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_key_has_no_row_stride(dim):
+    """One row of a very wide matrix as K and V: the distance to a row that is not there does not matter."""
+    wide = torch.zeros(2 ** 24 + 4 * dim, dtype=torch.float16, device="cuda")
+    kv = wide.as_strided((1, 2, dim), (2 ** 24, dim, 1))
+    kv.copy_(rand((1, 2, dim), 1, torch.float16))
+    q = rand((3, 2, dim), 2, torch.float16)
+    o = packed_attention(q, kv, kv, R.starts([3], "cuda"), R.starts([1], "cuda"), 3, 1, causal=False)
+    R.close(o, *R.attention(q, kv, kv, [3], [1], False))

@@ -30,3 +30,9 @@ def test_plan_names_the_kernel_and_fits_the_scratch(lib):
             ranges = plan(lib, paged, requests, rows, keys, hq, hkv, dim)[1]
             assert size(requests, rows, keys, hq, hkv, dim) == (ranges * requests * rows * hq * (dim + 2) * 4 if ranges > 1 else 0)
         assert [plan(lib, paged, *a) for a in ((0, 1, 1, 1, 1, 64), (1, 0, 1, 1, 1, 64), (1, 1, -1, 1, 1, 64), (1, 1, 1, 3, 2, 64), (1, 1, 1, 1, 1, 96))] == [-1] * 5
+
+
+def test_one_key_has_no_row_stride(lib):
+    """The limit of the row strides holds from two keys on (B = 0: nothing is launched)."""
+    call = lambda tk, rs: lib.iggt_packed_attn_f16(16, 64, 64, 16, rs, 64, 16, rs, 64, 16, 64, 64, 16, 16, 0, 4, tk, 4, 4, 1, 1, 64, 1.0, 1, 0, 0, 0)  # noqa: E731
+    assert call(1, 1 << 24) == 0 and call(2, 1 << 24) == -2 and call(2, (1 << 24) - 8) == 0 and call(1, (1 << 24) + 4) == -2
