@@ -59,7 +59,7 @@ IGGT_DEVINL void arrive() {
 // 932 us in place, 879 moved with every tile, 850 with every fourth, 845 every eighth: moving balances, staying shares the L2).
 template <bool PAGED>
 IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt, int& b, int& h) {
-    int w = blockIdx.x;
+    int w = (int)seq_item();
     if (p.causal || p.B == 1 || p.B > 64) {
         const int npairs = p.B * p.Hkv;
         int pair = w % npairs;
@@ -106,6 +106,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
     const int frow = lane & 31, fhalf = lane >> 5;
 
     int split, qt, b, h;
+    if (seq_item() >= p.items) return;
     work_item<PAGED>(p, lane, split, qt, b, h);
     const SeqSpan sp = seq_span<PAGED>(p, b);
     const long rows = (long)sp.lq * p.G;
@@ -666,7 +667,8 @@ int launch(const SeqAttnParams& p_in, hipStream_t stream) {
     p.qtiles = (int)(((long)p.max_q * p.G + BM - 1) / BM);
     const long n = (long)p.qtiles * p.splits * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
-    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, FMT, PAGED>), dim3((unsigned)n), dim3(64 * NW), 0, stream, p);
+    p.items = (unsigned)n;
+    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, FMT, PAGED>), seq_grid(n), dim3(64 * NW), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
 }

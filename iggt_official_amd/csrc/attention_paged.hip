@@ -41,7 +41,9 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
     const int npairs = p.B * p.Hkv;
     // (the 16-row tiles of one pair and key range lie npairs work items apart: with a multiple of 8 pairs on one XCD, and in any case
     // together in time, so that the codes come from memory once)
-    const int pair = blockIdx.x % npairs, rest = blockIdx.x / npairs;
+    const unsigned item = seq_item();
+    if (item >= p.items) return;
+    const int pair = item % npairs, rest = item / npairs;
     const int row0 = rest % p.qtiles * 16, split = rest / p.qtiles;
     const int b = pair / p.Hkv, h = pair - b * p.Hkv;
     const SeqSpan sp = seq_span<true>(p, b);
@@ -386,7 +388,8 @@ int launch_rows(const SeqAttnParams& p_in, int fmt, hipStream_t stream) {
     p.qtiles = (int)(((long)p.max_q * p.G + 15) / 16);
     const long n = (long)p.splits * p.qtiles * p.B * p.Hkv;
     if (n >= (1L << 31)) return -4;
-    const dim3 grid((unsigned)n), block(256);
+    p.items = (unsigned)n;
+    const dim3 grid = seq_grid(n), block(256);
     if (fmt == FMT_F16) {
         if (p.max_q == 1) hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_F16, false>), grid, block, 0, stream, p);
         else hipLaunchKernelGGL((seq_attn_rows_kernel<D, FMT_F16, true>), grid, block, 0, stream, p);

@@ -392,7 +392,7 @@ int append_h16(int fmt, const void* k, long k_rs, long k_hs, const void* v, long
                void* k_codes, void* k_scale, void* v_codes, void* v_scale, int num_pages, int page, int Hkv, int D, void* stream) {
     const int shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
     if (T < 0 || num_pages < 0 || shift < 0 || Hkv <= 0 || (D != 64 && D != 128)) return -1;
-    if (((long)num_pages << shift) >= (1L << 31) || Hkv > 131070 || T >= 0x7fffffff - 1024) return -1;
+    if (((long)num_pages << shift) >= (1L << 31) || Hkv > 131070 || T >= (1 << 30)) return -1;   // (grid: T / 64 x 256 threads)
     if ((k_rs | k_hs | v_rs | v_hs) % 8 || ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_codes | (uintptr_t)v_codes) % 16) return -2;
     if (T == 0 || num_pages == 0) return 0;
     AppendParams p = {(const uint16_t*)k, (const uint16_t*)v, k_rs, k_hs, v_rs, v_hs, slots, T, Hkv, num_pages << shift, shift,

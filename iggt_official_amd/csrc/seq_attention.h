@@ -32,11 +32,20 @@ struct SeqAttnParams {
     int B, Hq, Hkv, G, Tq, Tk, max_q, causal;
     int qtiles, splits;
     int range_blocks;     // few rows: key range of a split in blocks of 64 keys
+    unsigned items;       // work items; the grid may have more
     float scale_log2;     // softmax scale * log2(e)
     // splits > 1: key range s of a row leaves its unnormalised sum [splits][B][max_q][Hq][D] and (maximum, row sum) here
     float* part_o;
     float* part_ml;
 };
+
+// Grid of n < 2^31 work items and the item of a workgroup.  A grid's dimension may not have 2^32 threads: rows of 2^20 workgroups where
+// there are more (one long prompt among many thousand sequences).
+constexpr int GRID_ROW_LOG2 = 20;
+inline dim3 seq_grid(long n) {
+    return n <= (1L << GRID_ROW_LOG2) ? dim3((unsigned)n) : dim3(1u << GRID_ROW_LOG2, (unsigned)(((n - 1) >> GRID_ROW_LOG2) + 1));
+}
+IGGT_DEVINL unsigned seq_item() { return blockIdx.x + (blockIdx.y << GRID_ROW_LOG2); }
 
 constexpr float M_INIT = -3.0e38f;   // running maximum before the first key: finite, so that a masked score (-inf) gives 2^-inf = 0
 constexpr int FOLD_MAX = 64;         // key ranges a row is folded from at most

@@ -27,7 +27,7 @@ _INT, _BYTE = torch.int32, torch.uint8
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 MAX_REQUESTS = 8192
-MAX_ROWS = 2 ** 31 - 2 ** 20     # rows, keys, slots of a call: 32-bit numbers below the Python API
+MAX_ROWS = 2 ** 31 - 2 ** 20     # rows, keys, planned slots of a call: 32-bit numbers below the Python API
 
 
 # Calls of a few microseconds: conditions first, messages only where one fails, and no object that a plain number can stand for.
@@ -194,8 +194,8 @@ def append_pages(pages: Pages, k, v, slots):
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _refuse("append_pages is forward only: an input requires gradients")
     tokens = k.shape[0]
-    if tokens >= MAX_ROWS:
-        _refuse(f"fewer than {MAX_ROWS} tokens expected, got {tokens}")
+    if tokens >= 2 ** 30:
+        _refuse(f"fewer than 2^30 tokens expected, got {tokens}")
     _call(_APPEND, _APPEND_BF16 + (dtype == torch.float16), *_strides("k", k, 8), *_strides("v", v, 8),
           _index("slots", slots, tokens, where), tokens, pages.k_codes.data_ptr(), pages.k_scale.data_ptr(), pages.v_codes.data_ptr(),
           pages.v_scale.data_ptr(), n, page, heads, dim, _stream(where))

@@ -538,7 +538,7 @@ int iggt_paged_attn_f16(const void* q, long q_rs, long q_hs, void* o, long o_rs,
 /* What a call of these sizes runs, answered on the host (rows, ranges: host pointers): rows of a work item -- 16: a wave takes the
  * cached keys straight from memory; 128 / 256: tiles of keys in LDS -- and the number of key ranges that are folded afterwards (1: none). */
 int iggt_seq_attn_plan(int paged, int B, int max_q, int max_k, int Hq, int Hkv, int D, int* rows, int* ranges);
-/* Writes tokens 0 .. T - 1 (k / v like above) at slots[t] = page id * page + place (int32; outside the cache: token skipped).
+/* Writes tokens 0 .. T - 1 (T < 2^30, k / v like above) at slots[t] = page id * page + place (int32; outside the cache: token skipped).
  * Tokens of a page come as one run of consecutive slots per call, in order; places below the run's first are held tokens, those
  * above its last are not.  Scale of a page: the least 2^e with amax <= 448 * 2^e over the finite values, never below the one of
  * the tokens it holds (their codes are rewritten when it grows).  Infinities are written as the largest value, NaN as NaN. */

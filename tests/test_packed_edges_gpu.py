@@ -121,3 +121,29 @@ def test_one_key_has_no_row_stride(dim):
     q = rand((3, 2, dim), 2, torch.float16)
     o = packed_attention(q, kv, kv, R.starts([3], "cuda"), R.starts([1], "cuda"), 3, 1, causal=False)
     R.close(o, *R.attention(q, kv, kv, [3], [1], False))
+
+
+def test_packed_grid_of_more_than_32_bits_of_threads():
+    """One long prompt among 70 000 sequences of one token: 16 x 70 001 x 8 work items of 512 threads."""
+    n, heads, long = 70000, 8, 4000
+    lens = [1] * (n // 2) + [long] + [1] * (n // 2)
+    assert plan(False, n + 1, long, long, heads, heads, 64) == (256, 1)
+    q, k, v = (rand((n + long, heads, 64), i, torch.float16) for i in range(3))
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), torch.cumsum(torch.tensor(lens), 0)]).int().cuda()
+    o = packed_attention(q, k, v, cu, cu, long, long)
+    s = slice(n // 2, n // 2 + long)
+    R.close(o[s], *R.attention(q[s], k[s], v[s], [long], [long], True))
+    assert torch.equal(o[:n // 2], v[:n // 2]) and torch.equal(o[n // 2 + long:], v[n // 2 + long:])
+
+
+def test_cached_grid_of_more_than_32_bits_of_threads():
+    """A row for each of 2^20 + 1 requests of 16 heads, 256 threads each; all of them hold the same token."""
+    n, heads = 2 ** 20 + 1, 16
+    assert plan(True, n, 1, 1, heads, heads, 64) == (16, 1)
+    pages = Pages.empty(1, heads, 64, 16)
+    k, v = rand((1, heads, 64), 1, torch.float16), rand((1, heads, 64), 2, torch.float16)
+    append_pages(pages, k, v, ints([0]))
+    _, value = R.held(pages, ints([[0]]), [1])
+    q = torch.zeros(n, heads, 64, dtype=torch.float16, device="cuda")
+    o = paged_attention(q, pages, torch.zeros(n, 1, dtype=torch.int32, device="cuda"), torch.ones(n, dtype=torch.int32, device="cuda"), 1, 1)
+    assert (o == value.half()).all()

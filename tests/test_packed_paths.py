@@ -36,3 +36,9 @@ def test_one_key_has_no_row_stride(lib):
     """The limit of the row strides holds from two keys on (B = 0: nothing is launched)."""
     call = lambda tk, rs: lib.iggt_packed_attn_f16(16, 64, 64, 16, rs, 64, 16, rs, 64, 16, 64, 64, 16, 16, 0, 4, tk, 4, 4, 1, 1, 64, 1.0, 1, 0, 0, 0)  # noqa: E731
     assert call(1, 1 << 24) == 0 and call(2, 1 << 24) == -2 and call(2, (1 << 24) - 8) == 0 and call(1, (1 << 24) + 4) == -2
+
+
+def test_tokens_of_a_write_stay_below_2_to_the_30(lib):
+    """More would not be a grid; no pages: nothing is launched."""
+    call = lambda tokens: lib.iggt_append_pages_bf16(16, 64, 64, 16, 64, 64, 16, tokens, 16, 16, 16, 16, 0, 64, 1, 64, 0)  # noqa: E731
+    assert call(1 << 30) == -1 and call((1 << 30) - 1) == 0
