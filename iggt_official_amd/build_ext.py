@@ -21,11 +21,28 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
 
 
-def _stale(target, deps):
-    if not os.path.exists(target):
+def _stale(target, deps, cmd):
+    """Missing, older than what it is made of, or made by another command line (kept beside it)."""
+    if not os.path.exists(target) or not os.path.exists(target + ".cmd"):
         return True
     t = os.path.getmtime(target)
-    return any(os.path.getmtime(d) > t for d in deps)
+    with open(target + ".cmd") as f:
+        return f.read() != " ".join(cmd) or any(os.path.getmtime(d) > t for d in deps)
+
+
+def _start(target, cmd, verbose):
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    if os.path.exists(target + ".cmd"):
+        os.remove(target + ".cmd")
+    return target, cmd, subprocess.Popen(cmd)
+
+
+def _finish(target, cmd, process):
+    if process.wait() != 0:
+        raise RuntimeError(f"hipcc failed on {target}")
+    with open(target + ".cmd", "w") as f:
+        f.write(" ".join(cmd))
 
 
 def build(force=False, verbose=True):
@@ -34,23 +51,24 @@ def build(force=False, verbose=True):
     os.makedirs(obj_dir, exist_ok=True)
     headers = glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(HERE, "..", "include", "*.h"))
     headers.append(os.path.join(CSRC, "attention_v3.hip"))   # included by attention_v3_est.hip
-    objs, procs = [], []
+    objs, jobs = [], []
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        if force or _stale(obj, [src] + headers):
-            cmd = [HIPCC] + FLAGS + PER_FILE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            procs.append((src, subprocess.Popen(cmd)))
-    for src, pr in procs:
-        if pr.wait() != 0:
-            raise RuntimeError(f"hipcc failed on {src}")
-    if force or procs or _stale(LIB, objs):
-        cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+        cmd = [HIPCC] + FLAGS + PER_FILE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
+        if force or _stale(obj, [src] + headers, cmd):
+            jobs.append(_start(obj, cmd, verbose))
+    failed = []
+    for job in jobs:
+        try:
+            _finish(*job)
+        except RuntimeError as e:
+            failed.append(str(e))
+    if failed:
+        raise RuntimeError("; ".join(failed))
+    cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
+    if force or jobs or _stale(LIB, objs, cmd):
+        _finish(*_start(LIB, cmd, verbose))
     return LIB
 
 
