@@ -16,7 +16,7 @@
 //     pipe 81 % busy, matrix pipe 47 %.  4 sequences of up to 10 992 tokens, 16 heads, full, fp16: 1 207 - 1 240 us, 900 TFLOP/s, at a
 //     clock that this load pulls down to 1.7 GHz.  Two waves per SIMD with two query blocks each, offset against each other: the same
 //     there, 8 x 1 374 causal tokens 71 -> 57, 3 x 1 374 full 55 -> 48; pipelined over the tiles: 4 x 5 496 full 619 -> 590, 16 x 1 374
-//     causal 118 -> 100, but where less than two waves come to a SIMD up to 9 % faster (2 748 causal tokens 44 us, here 48).
+//     causal 118 -> 100.  Small grids run the pipelined form (launch_fmt).
 //   head dim 128: one query block, pipelined over the tiles.  Matrix and vector pipe 51 % each, 1.85 waves.  Prompts of 12 001 and 7 645
 //     tokens, 16 query and 4 key heads, causal, bf16: 800 - 830 us, 1 010 TFLOP/s at 1.95 GHz (a large library matrix product here:
 //     1 450).  Before the pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
@@ -88,16 +88,12 @@ IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt
     }
 }
 
-// Head dim 64, 16-bit keys: a wave needs 128 registers without a second tile's scores, so that four run on a SIMD and fill each other's
-// waits; the others have 256 and overlap matrix and vector work within a wave.
-constexpr int waves_per_simd(int D, int QB, bool PAGED) {
-    return D == 64 && QB == 1 && !PAGED ? 4 : 2;
-}
-
-template <int D, int QB, int NW, int FMT, bool PAGED>
-__global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_attn_tile_kernel(const SeqAttnParams p) {
+// Waves on a SIMD.  Two have 256 registers each and overlap matrix and vector work within a wave.  Head dim 64, 16-bit keys: without a
+// second tile's scores a wave needs 128, so that four run and fill each other's waits -- where there are as many (launch_fmt).
+template <int D, int QB, int NW, int FMT, bool PAGED, int WPS>
+__global__ __launch_bounds__(64 * NW, WPS) void seq_attn_tile_kernel(const SeqAttnParams p) {
     constexpr int ROWB = D * 2, K_BYTES = 64 * ROWB, TILE = 2 * K_BYTES, NKC = D / 16, NDH = D / 32, BM = 32 * NW * QB;
-    constexpr bool PIPELINED = QB == 1 && waves_per_simd(D, QB, PAGED) == 2;   // over the tiles
+    constexpr bool PIPELINED = QB == 1 && WPS == 2;   // over the tiles
     constexpr int NT = 64 * NW;   // threads
     constexpr int SLOTS = ROWB / 16;   // 16-byte slots of a K row
     __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
@@ -660,24 +656,34 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(D, QB, PAGED)) void seq_att
     }
 }
 
-template <int D, int QB, int NW, int FMT, bool PAGED>
+long items_of(const SeqAttnParams& p, int bm) { return ((long)p.max_q * p.G + bm - 1) / bm * p.splits * p.B * p.Hkv; }
+
+template <int D, int QB, int NW, int FMT, bool PAGED, int WPS = 2>
 int launch(const SeqAttnParams& p_in, hipStream_t stream) {
     SeqAttnParams p = p_in;
     constexpr int BM = 32 * NW * QB;
     p.qtiles = (int)(((long)p.max_q * p.G + BM - 1) / BM);
-    const long n = (long)p.qtiles * p.splits * p.B * p.Hkv;
+    const long n = items_of(p, BM);
     if (n >= (1L << 31)) return -4;
     p.items = (unsigned)n;
-    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, FMT, PAGED>), seq_grid(n), dim3(64 * NW), 0, stream, p);
+    hipLaunchKernelGGL((seq_attn_tile_kernel<D, QB, NW, FMT, PAGED, WPS>), seq_grid(n), dim3(64 * NW), 0, stream, p);
     IGGT_CHECK_LAUNCH();
     return 0;
 }
 
 template <int FMT, bool PAGED>
 int launch_fmt(const SeqAttnParams& p, int D, bool small, hipStream_t stream) {
-    if (small) return D == 64 ? launch<64, 1, 4, FMT, PAGED>(p, stream) : launch<128, 1, 4, FMT, PAGED>(p, stream);
-    if constexpr (PAGED) return D == 64 ? launch<64, 2, 4, FMT, PAGED>(p, stream) : launch<128, 1, 8, FMT, PAGED>(p, stream);
-    else return D == 64 ? launch<64, 1, 8, FMT, PAGED>(p, stream) : -1;    // (the plan has 128-row tiles for 128 channels)
+    if constexpr (PAGED) {
+        if (small) return D == 64 ? launch<64, 1, 4, FMT, PAGED>(p, stream) : launch<128, 1, 4, FMT, PAGED>(p, stream);
+        return D == 64 ? launch<64, 2, 4, FMT, PAGED>(p, stream) : launch<128, 1, 8, FMT, PAGED>(p, stream);
+    } else {
+        if (D == 128) return small ? launch<128, 1, 4, FMT, PAGED>(p, stream) : -1;    // (the plan has 128-row tiles for 128 channels)
+        // More than two waves per SIMD come of more than 512 work items.  Measured, 16 heads, four waves / two, pipelined over the tiles, us:
+        // full 700 tokens 16.4 / 14.8, 1 374 28.4 / 24.8, 2 x 1 374 (352 items) 37.7 / 36.2, 3 x 1 374 (528) 48.5 / 53.9, 4 122 (528)
+        // 122 / 133, 8 192 352 / 398; causal 1 374 28.1 / 25.4, 2 748 48.5 / 43.5, 4 x 1 374 34.0 / 38.4, 8 192 187 / 222 (but 4 122 72 / 65).
+        if (small) return items_of(p, 128) <= 512 ? launch<64, 1, 4, FMT, PAGED>(p, stream) : launch<64, 1, 4, FMT, PAGED, 4>(p, stream);
+        return launch<64, 1, 8, FMT, PAGED, 4>(p, stream);
+    }
 }
 
 }  // namespace

@@ -144,3 +144,18 @@ def test_every_key_at_a_tiles_end_counts_once(paged, item, split, dim, heads, n,
     ref, tol = R.attention(q, k, v, [lq], [n], causal)
     assert float(tol.max()) < 0.02 * float(ref.max())
     R.close(o, ref, tol)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,heads,lens", [(64, 2, [100, 300, 64]), (64, 80, [100, 300, 64]), (64, 640, [100, 7]), (64, 640, [128, 500]), (128, 2, [100, 300, 64]), (128, 640, [100, 7])])
+def test_packed_tiles_of_128_rows_on_small_and_full_grids(dim, heads, lens, causal, dt):
+    """64 channels: up to two waves per SIMD are pipelined over the tiles, more are not.  NaN among the values that only later rows see."""
+    lk = [n + 70 for n in lens]
+    if heads == 640:
+        lens = [min(n, 128) for n in lens]
+    assert plan(False, len(lens), max(lens), max(lk), heads, heads, dim) == (128, 1)
+    q, k, v = rand((sum(lens), heads, dim), 1, R.H16[dt], 1.5), rand((sum(lk), heads, dim), 2, R.H16[dt]), rand((sum(lk), heads, dim), 3, R.H16[dt])
+    v[lk[0] - 2, 0, 5], v[lk[0] - 1, heads - 1, 9], k[lk[0] - 1, 1, 2] = NAN, -INF, NAN
+    o = packed_attention(q, k, v, R.starts(lens, "cuda"), R.starts(lk, "cuda"), max(lens), max(lk), causal=causal)
+    R.close(o, *R.attention(q, k, v, lens, lk, causal))
