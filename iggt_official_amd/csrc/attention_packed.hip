@@ -76,7 +76,7 @@ IGGT_DEVINL void work_item(const SeqAttnParams& p, int lane, int& split, int& qt
         split = w % p.splits;
         w /= p.splits;
         qt = w % p.qtiles;
-        const int place = w / p.qtiles;
+        const int place = min(w / p.qtiles, p.B - 1);
         const int lk = lane < p.B ? seq_span<PAGED>(p, lane).lk : -1;
         int rank = 0;
         for (int i = 0; i < p.B; ++i) {
@@ -102,12 +102,11 @@ __global__ __launch_bounds__(64 * NW, WPS) void seq_attn_tile_kernel(const SeqAt
     const int frow = lane & 31, fhalf = lane >> 5;
 
     int split, qt, b, h;
-    if (seq_item() >= p.items) return;
     work_item<PAGED>(p, lane, split, qt, b, h);
     const SeqSpan sp = seq_span<PAGED>(p, b);
     const long rows = (long)sp.lq * p.G;
     const long row0 = (long)qt * BM;
-    if (row0 >= rows) return;
+    if (seq_item() >= p.items || row0 >= rows) return;   // (asked late: the arguments come in one go)
     auto limit_of = [&](long row) {   // keys that row sees
         return p.causal ? max(min(sp.lk, sp.off + (int)(row / p.G) + 1), 0) : sp.lk;
     };

@@ -42,13 +42,12 @@ __global__ __launch_bounds__(256, DRAFT ? 2 : 3) void seq_attn_rows_kernel(const
     // (the 16-row tiles of one pair and key range lie npairs work items apart: with a multiple of 8 pairs on one XCD, and in any case
     // together in time, so that the codes come from memory once)
     const unsigned item = seq_item();
-    if (item >= p.items) return;
     const int pair = item % npairs, rest = item / npairs;
     const int row0 = rest % p.qtiles * 16, split = rest / p.qtiles;
     const int b = pair / p.Hkv, h = pair - b * p.Hkv;
     const SeqSpan sp = seq_span<true>(p, b);
     const int rows = min(sp.lq * p.G - row0, 16);
-    if (rows <= 0) return;
+    if (item >= p.items || rows <= 0) return;   // (asked late: the arguments come in one go)
     const int first = p.causal ? max(min(sp.lk, sp.off + row0 / p.G + 1), 0) : sp.lk;    // keys that every row sees
     // keys that some row sees (one token: the same)
     const int kend = !DRAFT ? first : (p.causal ? max(min(sp.lk, sp.off + (row0 + rows - 1) / p.G + 1), 0) : sp.lk);

@@ -32,7 +32,7 @@ struct SeqAttnParams {
     int B, Hq, Hkv, G, Tq, Tk, max_q, causal;
     int qtiles, splits;
     int range_blocks;     // few rows: key range of a split in blocks of 64 keys
-    unsigned items;       // work items; the grid may have more
+    unsigned items;       // work items; the grid may have more (their sequence and key head exist all the same)
     float scale_log2;     // softmax scale * log2(e)
     // splits > 1: key range s of a row leaves its unnormalised sum [splits][B][max_q][Hq][D] and (maximum, row sum) here
     float* part_o;

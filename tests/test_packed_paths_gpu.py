@@ -159,3 +159,26 @@ def test_packed_tiles_of_128_rows_on_small_and_full_grids(dim, heads, lens, caus
     v[lk[0] - 2, 0, 5], v[lk[0] - 1, heads - 1, 9], k[lk[0] - 1, 1, 2] = NAN, -INF, NAN
     o = packed_attention(q, k, v, R.starts(lens, "cuda"), R.starts(lk, "cuda"), max(lens), max(lk), causal=causal)
     R.close(o, *R.attention(q, k, v, lens, lk, causal))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("page,heads,dim,tokens", [(64, 16, 64, 9000), (16, 17, 128, 9000), (128, 2, 64, 70000)])
+def test_append_pages_of_a_prompt_in_groups_of_64(page, heads, dim, tokens, dt):
+    """As many tokens and heads as make a workgroup look at 64 slots: whole pages in any order, rows that go nowhere in front."""
+    total = -(-tokens // page)
+    assert tokens // 64 * ((heads + 1) // 2) >= 1024
+    order = torch.randperm(total, generator=torch.Generator().manual_seed(1)).cuda()
+    t = torch.arange(tokens, device="cuda")
+    slots = (order[t // page] * page + t % page).int()
+    pages = Pages.empty(total, heads, dim, page)
+    kv = rand((tokens + 37, 2, heads, dim), 2, R.H16[dt], 3.0)
+    append_pages(pages, kv[:, 0], kv[:, 1], torch.cat([torch.full((37,), -1, dtype=torch.int32, device="cuda"), slots]))
+    k, v = (x.cuda() for x in R.code_values(pages))
+    for codes, byte, x in ((k, pages.k_scale, kv[37:, 0]), (v, pages.v_scale, kv[37:, 1])):
+        whole = torch.zeros(total * page, heads, dim, dtype=torch.float64, device="cuda")
+        whole[slots.long()] = x.double()
+        whole = whole.view(total, page, heads, dim).transpose(1, 2)
+        m, e = torch.frexp(whole.abs().amax((2, 3)))                     # 448 = 0.875 * 2^9
+        need = torch.where(m > 0, e - 9 + (m > 0.875).int() + 127, 1).clamp(1, 254)
+        assert torch.equal(byte.int(), need.int())
+        assert torch.equal(codes, R.e4m3(whole * torch.exp2(127.0 - need.double())[..., None, None]))
