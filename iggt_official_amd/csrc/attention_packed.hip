@@ -13,16 +13,18 @@
 //
 // What bounds it (MI355X):
 //   head dim 64, 16-bit keys: one query block per wave, nothing overlapped within it but four waves on a SIMD (128 registers).  Vector
-//     pipe 81 % busy, matrix pipe 47 %.  4 sequences of up to 10 992 tokens, 16 heads, full, fp16: 1 207 - 1 240 us, 900 TFLOP/s, at a
-//     clock that this load pulls down to 1.7 GHz.  Two waves per SIMD with two query blocks each, offset against each other: the same
+//     pipe 80 % busy, matrix pipe 48 %.  4 sequences of up to 10 992 tokens, 16 heads, full, fp16: 1 205 - 1 300 us between machines,
+//     850 - 910 TFLOP/s, at a clock that this load pulls down to 1.7 GHz; of the vector work the running maximum (its tree, exchange and
+//     vote) is what the trunk's kernel, which knows its shift beforehand, does without (1 080 - 1 120 TFLOP/s).  Two waves per SIMD with two query blocks each, offset against each other: the same
 //     there, 8 x 1 374 causal tokens 71 -> 57, 3 x 1 374 full 55 -> 48; pipelined over the tiles: 4 x 5 496 full 619 -> 590, 16 x 1 374
 //     causal 118 -> 100.  Small grids run the pipelined form (launch_fmt).
-//   head dim 128: one query block, pipelined over the tiles.  Matrix and vector pipe 51 % each, 1.85 waves.  Prompts of 12 001 and 7 645
-//     tokens, 16 query and 4 key heads, causal, bf16: 800 - 830 us, 1 010 TFLOP/s at 1.95 GHz (a large library matrix product here:
-//     1 450).  Before the pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
+//   head dim 128: one query block, pipelined over the tiles.  Matrix and vector pipe 50 % each, 1.8 waves.  Prompts of 12 001 and 7 645
+//     tokens, 16 query and 4 key heads, causal, bf16: 800 - 880 us, 940 - 1 040 TFLOP/s at 1.9 GHz (a large library matrix product here:
+//     1 430 - 1 450).  Before the pipeline and the fragments read ahead 970; eight waves and 256 rows per workgroup: 5 % slower.
 //   8-bit keys: the same with the conversion in front, shared by 256 rows where there are as many (head dim 64: two query blocks per
-//     wave, 128: eight waves).  1 374 rows against 12 366 tokens, 2 x 16 heads of 64, fp16: 228 us with the fold (one query block: 250),
-//     610 TFLOP/s; 6 x 1 374 rows against 36 343 tokens, 8 query and 2 key heads: 524 (607).
+//     wave, 128: eight waves).  1 374 rows against 12 366 tokens, 2 x 16 heads of 64, fp16: 205 - 240 us with the fold (one query block:
+//     + 10 %), 580 - 680 TFLOP/s; 6 x 1 374 rows against 36 343 tokens, 8 query and 2 key heads: 524 - 565 (+ 15 %).  Head dim 128, 5 x
+//     1 374 rows against <= 10 175 tokens, 8 heads: 322; 10 to 31 vector registers are spilled there.
 //   small grids: the chain of one wave's tiles, 0.8 us each; loads four tiles ahead instead of one change nothing.
 //
 // Values that are not finite: a masked score is replaced, not added to, so NaN in K costs nothing.  V does: 0 * inf = NaN in the
@@ -696,7 +698,8 @@ int iggt_launch_seq_tiles(const SeqAttnParams& p, int D, int fmt, bool paged, bo
 //   16-bit keys, head dim 64: 256 rows (eight waves) where they fill the chip twice (4 x 2 748 tokens, 16 heads, full: 171 -> 164 us, 2 x
 //   5 496 332 -> 309, but causal 8 x 1 374: 55 -> 57);
 //   8-bit keys: the workgroup converts the keys it reads, half of that work per row for 256 rows.  Head dim 128 (eight waves, whose
-//   coupling costs less than that: 1 374 rows against 10 175 tokens, 5 x 8 heads: 540 -> 420 us; with 16-bit keys 974 -> 1 033): more
+//   coupling costs less than that: 1 374 rows against 10 175 tokens, 5 x 8 heads: 540 -> 420 us before the spills went, 322 now; with
+//   16-bit keys 974 -> 1 033): more
 //   than 128 rows.  Head dim 64 (two query blocks per wave: 1 374 rows, 6 x 8 heads, 36 343 tokens 590 -> 525 us; 2 x 16 heads, 12 366
 //   tokens 250 -> 237; but 3 x 16 heads, 1 374 tokens, causal 33 -> 47, 4 heads, 2 748 tokens 24 -> 31): where the estimate below is lower.
 // Ranges, where the grid is small: the time of all items over the CUs, where the last CU to finish has between n and ceil(n) of n per CU

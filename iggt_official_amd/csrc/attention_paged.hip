@@ -14,7 +14,7 @@
 // softmax runs.  The four waves of a workgroup take every fourth block of its key range and are joined in LDS.
 // Measured (MI355X, a large copy moves 5.2 TB/s): one row, 350 784 tokens, 16 heads of 64: 123 us, 5.8 TB/s, + 5 us fold; 64 requests of
 // up to 8 192 tokens, 16 query and 4 key heads of 128: 60 us, 4.8 TB/s, + 5 us; one request of 1 374 tokens, 16 heads of 64, not split:
-// 7.5 us, the latency of five dependent loads and six blocks per wave.
+// 7.5 - 8.5 us, the latency of five dependent loads and six blocks per wave.
 #include "seq_attention.h"
 #include "../../include/iggt_hip.h"
 
@@ -402,8 +402,9 @@ int launch_rows(const SeqAttnParams& p_in, int fmt, hipStream_t stream) {
 
 // Few rows per (request, key head): the row kernel, a work item for every 16 of them.  Its own work grows with the 16-row tiles, the
 // tile kernel's hardly up to 128 rows, but that one reads and converts keys at a lower rate.  Measured, rows / tile kernel, us: 16
-// requests of 4 096 tokens, 4 key heads of 128: 32 rows 36 / 47, 64 rows 26 / 55, 128 rows 49 / 64; 32 requests of 2 048, 16 key heads of
-// 64: 32 rows 42 / 41, 64 rows 79 / 53; 2 of 16 384, 16 heads of 128: 64 rows 65 / 89, 128 rows 107 / 102.
+// requests of 4 096 tokens, 4 key heads of 128: 32 rows 36 / 33 (29 and a fold of 7), 64 rows 26 / 38 (not split), 128 rows 48 / 51; of 64:
+// 21 / 26, 18 / 25, 26 / 30; 32 requests of 2 048, 16 key heads of 64: 32 rows 41 / 53, 64 rows 76 / 53; of 128: 88 / 99, 154 / 92; 2 of
+// 16 384, 16 heads of 128: 64 rows 64 / 70, 128 rows 108 / 76.  (Few items, long: 40 000 tokens, 2 heads, 128 rows 19 / 31 and 31 / 51.)
 bool few_rows(int B, long max_q, long max_len, int Hkv, int G) {
     const long rows = max_q * G, items = (long)B * Hkv * ((rows + 15) / 16);
     return rows <= 32 || (items <= 1024 && (rows <= 64 || (rows <= 128 && max_len <= 4096)));

@@ -262,8 +262,8 @@ def _tables(tables, where, page):
 def plan_pages(tables, ring, counters, lens, new_lens, page: int, tokens: int):
     """One step of the block tables: requests that hold lens [R] tokens are to hold new_lens [R] (more: tokens are appended; fewer: the
     last ones are dropped; 0: the request ends).  Growing requests take pages from the head of `ring` [N] (free pages ring[(head + i) % N],
-    i < count; counters = (head, count, ...)), pages no longer needed go behind its tail for later steps, both in request order.
-    tables [R, width] and ring are updated in place; lens and counters are not.
+    i < count; counters = (head, count, ...)), pages no longer needed go behind its tail for later steps, both in request order.  Pages are
+    numbered 0 .. N - 1 (a token on any other has slot -1).  tables [R, width] and ring are updated in place; lens and counters are not.
 
     Returns (tables, ring, starts [R + 1], next_lens [R], next_counters [3] = (head, count, missing), slots [tokens]): slots of the
     added tokens in request order, -1 behind the last, request b's at starts[b] .. starts[b + 1].  `missing` pages > 0 (or -1: `tokens` is

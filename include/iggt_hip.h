@@ -551,6 +551,7 @@ int iggt_append_pages_f16(const void* k, long k_rs, long k_hs, const void* v, lo
 /* One step of the page tables (all int32 on the device): requests (<= 8192) hold lens[b] tokens and are to hold new_lens[b] (both
  * clamped to [0, table_width * page]).  Growing requests take pages off the ring of free pages (ring[(counters[0] + i) % num_pages],
  * i < counters[1]), shrinking ones put theirs behind its tail, both in request order; tables and ring are updated in place.
+ * Pages are numbered 0 .. num_pages - 1 (a token on any other has slot -1).
  *   slots [num_slots]: slot of every added token in request order, -1 behind the last;  starts [requests + 1]: its prefix sums
  *   next_lens [requests], next_counters [3]: lengths, (head, free pages) after the step, and the number of pages that were missing
  * With pages missing, or -1 (num_slots too short), no request grows in this step.  Outputs do not overlap the inputs. */
