@@ -15,7 +15,7 @@
 //   head dim 64, 16-bit keys: one query block per wave, nothing overlapped within it but four waves on a SIMD (128 registers).  Vector
 //     pipe 80 % busy, matrix pipe 48 %.  4 sequences of up to 10 992 tokens, 16 heads, full, fp16: 1 205 - 1 300 us between machines,
 //     850 - 910 TFLOP/s, at a clock that this load pulls down to 1.7 GHz; of the vector work the running maximum (its tree, exchange and
-//     vote) is what the trunk's kernel, which knows its shift beforehand, does without (1 080 - 1 120 TFLOP/s).  Two waves per SIMD with two query blocks each, offset against each other: the same
+//     vote) is what the trunk's kernel, which knows its shift beforehand, does without (1 080 - 1 130 TFLOP/s).  Two waves per SIMD with two query blocks each, offset against each other: the same
 //     there, 8 x 1 374 causal tokens 71 -> 57, 3 x 1 374 full 55 -> 48; pipelined over the tiles: 4 x 5 496 full 619 -> 590, 16 x 1 374
 //     causal 118 -> 100.  Small grids run the pipelined form (launch_fmt).
 //   head dim 128: one query block, pipelined over the tiles.  Matrix and vector pipe 50 % each, 1.8 waves.  Prompts of 12 001 and 7 645

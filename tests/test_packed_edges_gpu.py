@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import packed_ref as R
-from iggt_official_amd.layers import Pages, append_pages, packed_attention, paged_attention
+from iggt_official_amd.layers import Pages, append_pages, packed_attention, paged_attention, plan_pages
 from test_packed_gpu import INF, NAN, ints, make_cache, rand
 from test_packed_paths_gpu import cached, plan
 
@@ -147,3 +147,23 @@ def test_cached_grid_of_more_than_32_bits_of_threads():
     q = torch.zeros(n, heads, 64, dtype=torch.float16, device="cuda")
     o = paged_attention(q, pages, torch.zeros(n, 1, dtype=torch.int32, device="cuda"), torch.ones(n, dtype=torch.int32, device="cuda"), 1, 1)
     assert (o == value.half()).all()
+
+
+def test_planner_of_many_requests_in_a_captured_graph():
+    """More requests than the default of dynamic LDS holds: captured, and replayed with eager work in between, it plans what an eager call does."""
+    n, page, width = 5000, 16, 3
+    new = ints([(7 * i) % 49 for i in range(n)])
+    state = [torch.full((n, width), -1, dtype=torch.int32, device="cuda"), torch.randperm(3 * n).int().cuda(), ints([0, 3 * n]), ints([0] * n)]
+    first = [t.clone() for t in state]
+    want = [t.clone() for t in plan_pages(*state, new, page, 49 * n)]
+    for t, old in zip(state, first):
+        t.copy_(old)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = plan_pages(*state, new, page, 49 * n)
+    for _ in range(3):
+        for t, old in zip(state, first):
+            t.copy_(old)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
